@@ -1,0 +1,429 @@
+// Selection over beams and vocabulary: one step of a draft (or of a beam
+// search), with the beams' states put in the order of the selected parents.
+//
+// With x = logits[b, w, :] and c = scores[b, w],
+//   value(w, v) = (c + x[v]) - lse_w,   lse_w = log sum_v exp(x[v]),
+// the k best (w, v) of every b by value, ties to the lowest w * vocab + v.
+// Values are formed and compared in 64 bits: with tens of candidates per unit
+// of value, 32-bit rounding of lse swaps neighbours of different beams about
+// once in some hundred calls.  Within a beam the order is that of the logits,
+// so the vocabulary pass keeps k candidates by logit alone and needs no lse:
+//   part_kernel   one workgroup per tile of a row: the tile's maximum, its sum
+//                 of exponentials (64 bit) and its k best, one pass over the
+//                 logits, which stay in registers;
+//   merge_kernel  one workgroup per b: lse of every beam, the k best of the
+//                 tiles' candidates;
+//   states_kernel the states' rows of the selected parents.
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+
+#include "tsfa_internal.h"
+
+namespace tsfa {
+namespace beam {
+
+constexpr int kThreads = 256;
+constexpr int kMaxK = 64;
+constexpr int kMaxBeams = 256;
+constexpr int kMaxStates = 8;
+
+// Statistics of one tile: maximum (as a float) and sum of exp(x - maximum).
+struct PartStat {
+  double sum;
+  float top;
+  int pad;
+};
+
+struct PartArgs {
+  const void* logits;
+  int64_t sb, sw;  // strides of sequence and beam, in elements
+  int beams, vocab, k, tiles;
+  uint64_t* keys;   // [rows][tiles][k], best first, 0: none
+  PartStat* stats;  // [rows][tiles]
+};
+
+// A candidate of a row as one number, better = larger: the logit in an order
+// of its bits that integers compare alike (-0 counts as 0), then the lower
+// token.  0 is no candidate (-inf, NaN, past the row).
+__device__ inline uint64_t make_key(float x, uint32_t v) {
+  if (!(x > -INFINITY)) return 0;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return ((uint64_t)o << 32) | (uint32_t)~v;
+}
+__device__ inline float key_logit(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ inline uint32_t key_token(uint64_t key) { return ~(uint32_t)key; }
+
+// exp(x - top) for x <= top, with exp(0) also for equal infinities.
+__device__ inline double weight(float x, float top) {
+  if (x == top) return 1.0;
+  return exp((double)x - (double)top);
+}
+
+// EPT elements per thread, VEC of them in one 16-byte load.
+template <typename T, int EPT>
+__global__ __launch_bounds__(kThreads) void part_kernel(const PartArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T), NU = EPT / VEC;
+  __shared__ __attribute__((aligned(16))) uint64_t best[kThreads];
+  __shared__ uint64_t list[kMaxK * EPT];
+  __shared__ double wsum[kThreads / 64];
+  __shared__ float wtop[kThreads / 64];
+  __shared__ uint64_t bound;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tile = blockIdx.x % a.tiles, row = blockIdx.x / a.tiles;
+  const int b = row / a.beams, w = row - b * a.beams;
+  const T* x = static_cast<const T*>(a.logits) + b * a.sb + w * a.sw;
+  const int v0 = tile * (kThreads * EPT);
+
+  float xs[EPT];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    const int v = v0 + (u * kThreads + tid) * VEC;
+    if (v + VEC <= a.vocab) {
+      T t[VEC];
+      __builtin_memcpy(t, x + v, 16);  // rows of an odd vocabulary start anywhere
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) xs[u * VEC + j] = (float)t[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) xs[u * VEC + j] = v + j < a.vocab ? (float)x[v + j] : -INFINITY;
+    }
+  }
+  auto token = [&](int e) { return (uint32_t)(v0 + ((e / VEC) * kThreads + tid) * VEC + e % VEC); };
+
+  if (tid == 0) {
+    bound = 1;  // fewer than k threads hold a candidate: all of them
+    count = 0;
+  }
+  float top = -INFINITY;
+  uint64_t mine = 0;
+#pragma unroll
+  for (int e = 0; e < EPT; ++e) {
+    if (!(xs[e] == xs[e])) xs[e] = -INFINITY;  // NaN is no candidate and weighs nothing
+    top = fmaxf(top, xs[e]);
+    const uint64_t key = make_key(xs[e], token(e));
+    mine = key > mine ? key : mine;
+  }
+  best[tid] = mine;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+  if (lane == 0) wtop[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) top = fmaxf(top, wtop[i]);
+
+  double sum = 0;
+  if (top > -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) sum += weight(xs[e], top);
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+  if (lane == 0) wsum[wave] = sum;
+
+  // The k-th best of the threads' best bounds the tile's k-th best from below,
+  // and only the k threads at or above it hold anything better: at most k *
+  // EPT elements whatever the values are.
+  if (mine != 0) {
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < kThreads; ++i) rank += best[i] > mine;
+    if (rank == a.k - 1) bound = mine;
+  }
+  __syncthreads();
+  const uint64_t lim = bound;
+  if (mine >= lim) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) {
+      const uint64_t key = make_key(xs[e], token(e));
+      if (key >= lim) list[atomicAdd(&count, 1)] = key;
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  uint64_t* out = a.keys + ((int64_t)row * a.tiles + tile) * a.k;
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t key = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > key;
+    if (rank < a.k) out[rank] = key;
+  }
+  for (int i = n + tid; i < a.k; i += kThreads) out[i] = 0;
+  if (tid == 0) {
+    PartStat st;
+    st.sum = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) st.sum += wsum[i];
+    st.top = top;
+    st.pad = 0;
+    a.stats[(int64_t)row * a.tiles + tile] = st;
+  }
+}
+
+struct MergeArgs {
+  const uint64_t* keys;
+  const PartStat* stats;
+  const float* scores;  // [batch][beams]
+  int64_t ssb, ssw;
+  int beams, vocab, k, tiles;
+  int64_t* tokens;
+  int64_t* parents;
+  float* out_scores;
+};
+
+// A candidate over all beams: value, then the lower w * vocab + v.  None: -inf.
+struct Cand {
+  double value;
+  uint32_t flat, pad;
+};
+__device__ inline bool better(const Cand& x, const Cand& y) {
+  return x.value > y.value || (x.value == y.value && x.flat < y.flat);
+}
+
+constexpr int kBatch = 4;  // candidates per thread and round
+
+__global__ __launch_bounds__(kThreads) void merge_kernel(const MergeArgs a) {
+  __shared__ double lse[kMaxBeams], score[kMaxBeams];
+  __shared__ float tops[kMaxBeams];
+  __shared__ Cand heads[kThreads];
+  __shared__ Cand list[kMaxK * kBatch + kMaxK];
+  __shared__ Cand kept[kMaxK];
+  __shared__ Cand bound;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x;
+  const Cand none = {-INFINITY, 0xffffffffu, 0};
+
+  // lse_w = top + log(sum) of the tiles; a beam with no finite or infinite
+  // logit, or whose score is not finite, has no candidates
+  for (int w = wave; w < a.beams; w += kThreads / 64) {
+    const PartStat* st = a.stats + ((int64_t)b * a.beams + w) * a.tiles;
+    float top = -INFINITY;
+    for (int i = lane; i < a.tiles; i += 64) top = fmaxf(top, st[i].top);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+    double sum = 0;
+    for (int i = lane; i < a.tiles; i += 64)
+      if (st[i].top > -INFINITY) sum += st[i].sum * weight(st[i].top, top);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+    if (lane == 0) {
+      const float c = a.scores[b * a.ssb + w * a.ssw];
+      const bool alive = top > -INFINITY && c - c == 0.0f;
+      tops[w] = top;
+      score[w] = alive ? (double)c : -INFINITY;
+      // tokens at +inf share the beam's mass: their own logit and the
+      // maximum cancel
+      lse[w] = top < INFINITY ? (double)top + log(sum) : log(sum);
+    }
+  }
+  for (int i = tid; i < a.k; i += kThreads) kept[i] = none;
+  __syncthreads();
+
+  // Candidates in rounds, the tiles' best first, so that the first rounds
+  // bring the bound near its end and the later ones find little above it.
+  const int lists = a.beams * a.tiles;
+  const int64_t total = (int64_t)lists * a.k;
+  const uint64_t* keys = a.keys + (int64_t)b * lists * a.k;
+  for (int64_t c0 = 0; c0 < total; c0 += kThreads * kBatch) {
+    const Cand last = kept[a.k - 1];
+    Cand cs[kBatch], top = none;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t c = c0 + j * kThreads + tid;
+      cs[j] = none;
+      if (c < total) {
+        const int p = (int)(c / lists), l = (int)(c - (int64_t)p * lists);
+        const uint64_t key = keys[(int64_t)l * a.k + p];
+        const int w = l / a.tiles;
+        if (key != 0 && score[w] > -INFINITY) {
+          const float x = key_logit(key);
+          const bool inf = tops[w] == INFINITY;
+          if (!inf || x == INFINITY) {
+            cs[j].value = (score[w] + (inf ? 0.0 : (double)x)) - lse[w];
+            cs[j].flat = (uint32_t)w * (uint32_t)a.vocab + key_token(key);
+          }
+        }
+      }
+      if (!better(cs[j], last)) cs[j] = none;
+      if (better(cs[j], top)) top = cs[j];
+    }
+    heads[tid] = top;
+    if (tid == 0) {
+      bound = last;
+      count = 0;
+    }
+    if (__syncthreads_or(top.value > -INFINITY) == 0) continue;
+    if (top.value > -INFINITY) {
+      int rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < kThreads; ++i) rank += better(heads[i], top);
+      if (rank == a.k - 1) bound = top;  // k candidates at least as good
+    }
+    __syncthreads();
+    const Cand lim = bound;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (cs[j].value > -INFINITY && !better(lim, cs[j])) list[atomicAdd(&count, 1)] = cs[j];
+    __syncthreads();
+    const int n = count;
+    // the kept ones join, all are ranked, the k best stay
+    for (int i = tid; i < a.k; i += kThreads) list[n + i] = kept[i];
+    __syncthreads();
+    for (int i = tid; i < n + a.k; i += kThreads) {
+      const Cand x = list[i];
+      if (x.value == -INFINITY) continue;
+      int rank = 0;
+      for (int j = 0; j < n + a.k; ++j) rank += better(list[j], x);
+      if (rank < a.k) kept[rank] = x;
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < a.k; i += kThreads) {
+    const Cand x = kept[i];
+    const bool ok = x.value > -INFINITY;
+    const int64_t at = (int64_t)b * a.k + i;
+    a.tokens[at] = ok ? (int64_t)(x.flat % (uint32_t)a.vocab) : 0;
+    a.parents[at] = ok ? (int64_t)(x.flat / (uint32_t)a.vocab) : 0;
+    a.out_scores[at] = ok ? (float)x.value : -INFINITY;
+  }
+}
+
+struct StatesArgs {
+  const void* src[kMaxStates];
+  void* dst[kMaxStates];
+  int64_t row_bytes[kMaxStates];
+  const int64_t* parents;  // [batch][k]
+  int beams, k;
+};
+
+__global__ __launch_bounds__(kThreads) void states_kernel(const StatesArgs a) {
+  const int s = blockIdx.z, at = blockIdx.y;
+  const int64_t bytes = a.row_bytes[s];
+  const char* src = static_cast<const char*>(a.src[s]) + ((int64_t)(at / a.k) * a.beams + a.parents[at]) * bytes;
+  char* dst = static_cast<char*>(a.dst[s]) + (int64_t)at * bytes;
+  const int64_t i0 = (int64_t)blockIdx.x * kThreads + threadIdx.x, step = (int64_t)gridDim.x * kThreads;
+  if (((reinterpret_cast<uintptr_t>(a.src[s]) | reinterpret_cast<uintptr_t>(a.dst[s]) | (uintptr_t)bytes) & 15) == 0) {
+    for (int64_t i = i0; i < bytes / 16; i += step)
+      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+  } else {
+    for (int64_t i = i0; i < bytes; i += step) dst[i] = src[i];
+  }
+}
+
+// Elements of a tile per thread: long tiles where the rows alone fill the
+// card, short ones where a row has to be spread over it.
+inline int elements_per_thread(int64_t rows, int vocab) {
+  const int64_t long_tiles = ((int64_t)vocab + kThreads * 32 - 1) / (kThreads * 32);
+  return rows * long_tiles >= 1024 ? 32 : 8;
+}
+inline int64_t tiles_of(int64_t rows, int vocab) {
+  const int64_t n = (int64_t)kThreads * elements_per_thread(rows, vocab);
+  return (vocab + n - 1) / n;
+}
+
+int check(int batch, int beams, int vocab, int k, int dtype) {
+  if (batch < 0 || beams <= 0 || vocab <= 0 || k <= 0) return TSFA_ERR_INVALID_ARGUMENT;
+  if ((int64_t)k > (int64_t)beams * vocab) return TSFA_ERR_INVALID_ARGUMENT;
+  if (dtype != TSFA_DTYPE_FP16 && dtype != TSFA_DTYPE_BF16 && dtype != TSFA_DTYPE_FP32) return TSFA_ERR_UNSUPPORTED;
+  if (k > kMaxK || beams > kMaxBeams || (int64_t)beams * vocab > (1 << 30)) return TSFA_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)batch * beams;
+  if ((int64_t)batch * k > 65535 || rows * tiles_of(rows, vocab) > INT32_MAX) return TSFA_ERR_UNSUPPORTED;
+  return TSFA_OK;
+}
+
+template <typename T> void launch_part(const PartArgs& a, int ept, int64_t rows, hipStream_t s) {
+  const dim3 grid((unsigned)(rows * a.tiles));
+  if (ept == 32) hipLaunchKernelGGL((part_kernel<T, 32>), grid, dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((part_kernel<T, 8>), grid, dim3(kThreads), 0, s, a);
+}
+
+}  // namespace beam
+}  // namespace tsfa
+
+using namespace tsfa;
+using namespace tsfa::beam;
+
+extern "C" size_t tsfa_beam_select_workspace_bytes(int batch, int beams, int vocab, int k) {
+  if (beam::check(batch, beams, vocab, k, TSFA_DTYPE_FP32) != TSFA_OK || batch == 0) return 0;
+  const int64_t rows = (int64_t)batch * beams, parts = rows * tiles_of(rows, vocab);
+  return align256((size_t)parts * k * sizeof(uint64_t)) + align256((size_t)parts * sizeof(PartStat));
+}
+
+extern "C" int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, int64_t logits_beam_stride,
+                                const float* scores, int64_t scores_seq_stride, int64_t scores_beam_stride, int batch,
+                                int beams, int vocab, int k, int dtype, int64_t* tokens, int64_t* parents,
+                                float* out_scores, const void* const* states, void* const* out_states,
+                                const int64_t* state_row_bytes, int n_states, void* workspace, size_t workspace_bytes,
+                                tsfa_stream_t stream) {
+  const int st = beam::check(batch, beams, vocab, k, dtype);
+  if (st != TSFA_OK) return st;
+  if (n_states < 0) return TSFA_ERR_INVALID_ARGUMENT;
+  if (n_states > kMaxStates) return TSFA_ERR_UNSUPPORTED;
+  if (batch == 0) return TSFA_OK;
+  if (logits == nullptr || scores == nullptr || tokens == nullptr || parents == nullptr || out_scores == nullptr)
+    return TSFA_ERR_INVALID_ARGUMENT;
+  StatesArgs sa;
+  int64_t most = 0;
+  for (int i = 0; i < n_states; ++i) {
+    if (states == nullptr || out_states == nullptr || state_row_bytes == nullptr || state_row_bytes[i] < 0)
+      return TSFA_ERR_INVALID_ARGUMENT;
+    if (state_row_bytes[i] > 0 && (states[i] == nullptr || out_states[i] == nullptr)) return TSFA_ERR_INVALID_ARGUMENT;
+    sa.src[i] = states[i];
+    sa.dst[i] = out_states[i];
+    sa.row_bytes[i] = state_row_bytes[i];
+    most = state_row_bytes[i] > most ? state_row_bytes[i] : most;
+  }
+  const int64_t rows = (int64_t)batch * beams;
+  const int ept = elements_per_thread(rows, vocab);
+  const int64_t tiles = tiles_of(rows, vocab), parts = rows * tiles;
+  const size_t key_bytes = align256((size_t)parts * k * sizeof(uint64_t));
+  if (workspace == nullptr || workspace_bytes < key_bytes + align256((size_t)parts * sizeof(PartStat)) ||
+      reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return TSFA_ERR_WORKSPACE;
+
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  PartArgs pa;
+  pa.logits = logits;
+  pa.sb = logits_seq_stride;
+  pa.sw = logits_beam_stride;
+  pa.beams = beams;
+  pa.vocab = vocab;
+  pa.k = k;
+  pa.tiles = (int)tiles;
+  pa.keys = static_cast<uint64_t*>(workspace);
+  pa.stats = reinterpret_cast<PartStat*>(static_cast<char*>(workspace) + key_bytes);
+  if (dtype == TSFA_DTYPE_BF16) launch_part<__bf16>(pa, ept, rows, s);
+  else if (dtype == TSFA_DTYPE_FP16) launch_part<_Float16>(pa, ept, rows, s);
+  else launch_part<float>(pa, ept, rows, s);
+
+  MergeArgs ma;
+  ma.keys = pa.keys;
+  ma.stats = pa.stats;
+  ma.scores = scores;
+  ma.ssb = scores_seq_stride;
+  ma.ssw = scores_beam_stride;
+  ma.beams = beams;
+  ma.vocab = vocab;
+  ma.k = k;
+  ma.tiles = (int)tiles;
+  ma.tokens = tokens;
+  ma.parents = parents;
+  ma.out_scores = out_scores;
+  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)batch), dim3(kThreads), 0, s, ma);
+
+  if (most > 0) {
+    sa.parents = parents;
+    sa.beams = beams;
+    sa.k = k;
+    const int64_t blocks = (most / 16 + kThreads) / kThreads;
+    hipLaunchKernelGGL(states_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), (unsigned)(batch * k), (unsigned)n_states),
+                       dim3(kThreads), 0, s, sa);
+  }
+  return hipGetLastError() == hipSuccess ? TSFA_OK : TSFA_ERR_LAUNCH;
+}

@@ -23,13 +23,19 @@ Extensions (no reference counterpart):
   tree_sparse_attention_fwd_paged: the same forward over a paged K/V cache
   (FlashInfer's [pages, 2, page_size, Hkv, D] layout, benchmark.py:67-91)
   with per-sequence page lists, read in place.
+  Serving over that cache, sequences of different lengths, all lengths on the
+  device: beam_select (one step of a draft: the best continuations over beams
+  and vocabulary, states reordered), append_paged_kv (queries and keys rotated
+  by their positions, keys and values written to their pages),
+  tree_sparse_attention_fwd_paged_varlen (the drafted tokens' attention).
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass, field
-from typing import List, Optional
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -774,3 +780,299 @@ def tree_sparse_attention_fwd_paged(q: torch.Tensor, kv_cache: torch.Tensor, kv_
             _lib.i64_array(out.stride()), float(sm_scale), *args, _lib.ptr(ws), ws_bytes, _lib.stream_handle(dev))
     _lib.check("tree_sparse_attention_fwd_paged", st)
     return (out, lse) if return_lse else out
+
+
+# ------------------------------------------------- serving over the paged cache
+def _paged_pool(kv_cache: torch.Tensor, kv_layout: str):
+    """(pages, page_size, kv heads, head_dim, strides as page/slot/row/head/d) of a paged cache."""
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2:
+        raise ValueError("kv_cache must be [pages, 2, page_size, Hkv, D] (NHD) or [pages, 2, Hkv, page_size, D] (HND)")
+    sp, ss, s2, s3, sd = kv_cache.stride()
+    if kv_layout == "NHD":
+        n_pages, _, page_size, n_kv_heads, d = kv_cache.shape
+        return n_pages, page_size, n_kv_heads, d, (sp, ss, s2, s3, sd)
+    if kv_layout == "HND":
+        n_pages, _, n_kv_heads, page_size, d = kv_cache.shape
+        return n_pages, page_size, n_kv_heads, d, (sp, ss, s3, s2, sd)
+    raise ValueError(f"kv_layout must be 'NHD' or 'HND', got {kv_layout!r}")
+
+
+def _varlen_lists(q_indptr, kv_lens, kv_indices, kv_indptr, page_size):
+    """Checks of the lengths and page lists; (batch, kv_indices, stride and width of a dense table)."""
+    for name, t in (("q_indptr", q_indptr), ("kv_lens", kv_lens), ("kv_indices", kv_indices), ("kv_indptr", kv_indptr)):
+        if t is not None and t.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32")
+    if kv_lens.dim() != 1 or q_indptr.dim() != 1 or q_indptr.numel() != kv_lens.numel() + 1:
+        raise ValueError(f"kv_lens must be [B] and q_indptr [B + 1], got {tuple(kv_lens.shape)} and "
+                         f"{tuple(q_indptr.shape)}")
+    batch = kv_lens.numel()
+    if page_size < 16 or page_size & (page_size - 1):
+        raise NotImplementedError(f"page_size must be a power of two >= 16, got {page_size}")
+    if kv_indptr is not None:
+        if kv_indptr.dim() != 1 or kv_indptr.numel() != batch + 1:
+            raise ValueError(f"kv_indptr must be int32 [{batch + 1}]")
+        return batch, kv_indices.contiguous().view(-1), 0, 0
+    if kv_indices.dim() != 2 or kv_indices.shape[0] != batch:
+        raise ValueError(f"a dense page table must be [{batch}, pages_per_seq] int32")
+    if kv_indices.stride(1) != 1 or kv_indices.stride(0) < kv_indices.shape[1]:
+        kv_indices = kv_indices.contiguous()
+    return batch, kv_indices, kv_indices.stride(0), kv_indices.shape[1]
+
+
+def _table_entries(kv_indices: torch.Tensor) -> int:
+    # entries from the first to the last of a (row-strided) dense table
+    if kv_indices.dim() == 1 or kv_indices.shape[0] == 0:
+        return kv_indices.numel()
+    return (kv_indices.shape[0] - 1) * kv_indices.stride(0) + kv_indices.shape[1]
+
+
+def _same_device(dev, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a HIP device tensor")
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}")
+
+
+def _run_on(dev, name: str, launch) -> None:
+    # the device guard only when the tensors are not on the current device (~1.2 us)
+    if dev.index == torch.cuda.current_device():
+        st = launch(_lib.stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = launch(_lib.stream_handle(dev))
+    _lib.check(name, st)
+
+
+def _packed_heads(name: str, t: torch.Tensor, tokens: int, head_dim: int) -> None:
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != head_dim:
+        raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}], got {tuple(t.shape)}")
+
+
+def append_paged_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
+                    kv_indices: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+                    q_indptr: torch.Tensor, kv_lens: torch.Tensor, kv_indptr: Optional[torch.Tensor] = None,
+                    kv_layout: str = "NHD", interleaved: bool = False, attention_scaling: float = 1.0,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate q and k by their positions, write k and v into the paged cache; returns the rotated q.
+
+    q [N, Hq, D], k and v [N, Hkv, D]: the tokens of all sequences, packed;
+        sequence b owns rows q_indptr[b] .. q_indptr[b + 1] - 1 (int32
+        [B + 1]).  Views of a fused projection are read in place.
+    kv_cache, kv_indices, kv_indptr, kv_layout: the pool and page lists of
+        tree_sparse_attention_fwd_paged, a list as long as its sequence needs.
+    kv_lens: int32 [B], keys of each sequence with these tokens appended:
+        token i of sequence b becomes key kv_lens[b] - q_len + i.
+    positions: int64 or int32 [N], the tokens' positions (a drafted token's is
+        the prefix length plus its depth in the tree).
+    inv_freq: float32 [rot / 2]: pair i of the first rot elements of a head
+        turns by positions * inv_freq[i], formed in 64 bits; rot may be below
+        D (the rest is copied) or 0.  Pairs are (i, rot / 2 + i), or (2i,
+        2i + 1) with ``interleaved``; ``attention_scaling`` multiplies the
+        rotated elements.
+    out: where the rotated q goes (q itself: in place); allocated otherwise.
+    Tokens behind q_indptr[B] are left as they were, in ``out`` and the cache;
+    a token whose place is outside its list or the pool is not written.  Two
+    tokens must not share a place.  No host synchronisation; nothing about the
+    lengths is checked on the host.
+    """
+    n_pages, page_size, n_kv_heads, head_dim, cache_strides = _paged_pool(kv_cache, kv_layout)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [N, Hq, D], got {tuple(q.shape)}")
+    n, n_heads = q.shape[0], q.shape[1]
+    _packed_heads("q", q, n, head_dim)
+    _packed_heads("k", k, n, head_dim)
+    _packed_heads("v", v, n, head_dim)
+    if k.shape[1] != n_kv_heads or v.shape[1] != n_kv_heads:
+        raise ValueError(f"k and v must have the cache's {n_kv_heads} heads")
+    if out is not None and tuple(out.shape) != tuple(q.shape):
+        raise ValueError(f"out shape {tuple(out.shape)} != q shape {tuple(q.shape)}")
+    if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) != (n,):
+        raise ValueError(f"positions must be int64 or int32 [{n}]")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be float32 [rot / 2]")
+    if not math.isfinite(attention_scaling):
+        raise ValueError("attention_scaling must be finite")
+    batch, kv_indices, pt_stride, pt_width = _varlen_lists(q_indptr, kv_lens, kv_indices, kv_indptr, page_size)
+    if not (q.dtype == k.dtype == v.dtype == kv_cache.dtype) or (out is not None and out.dtype != q.dtype):
+        raise NotImplementedError("q, k, v, kv_cache and out must share one dtype")
+    dt = _lib.dtype_code(q.dtype)
+    dev = q.device
+    _same_device(dev, q=q, k=k, v=v, kv_cache=kv_cache, kv_indices=kv_indices, kv_indptr=kv_indptr, q_indptr=q_indptr,
+                 kv_lens=kv_lens, positions=positions, inv_freq=inv_freq, out=out)
+    qc, k, v = _row_contig(q), _row_contig(k), _row_contig(v)
+    target = torch.empty_like(qc) if out is None else out
+    dst = target if _layout_ok(target) else target.contiguous()
+    lib = _lib.load()
+    args = (batch, n, n_heads, n_kv_heads, head_dim, dt)
+    q_indptr, kv_lens, positions, inv_freq = (t.contiguous() for t in (q_indptr, kv_lens, positions, inv_freq))
+    kv_indptr = None if kv_indptr is None else kv_indptr.contiguous()
+    _run_on(dev, "append_paged_kv", lambda stream: lib.tsfa_append_paged_kv(
+        qc.data_ptr(), k.data_ptr(), v.data_ptr(), dst.data_ptr(), kv_cache.data_ptr(), positions.data_ptr(),
+        int(positions.dtype == torch.int64), inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved),
+        float(attention_scaling), q_indptr.data_ptr(), kv_lens.data_ptr(), _lib.ptr(kv_indptr), kv_indices.data_ptr(),
+        _table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size,
+        _lib.i64_array((*qc.stride(), *k.stride(), *v.stride(), *dst.stride())), _lib.i64_array(cache_strides), *args,
+        stream))
+    if dst is not target:
+        target.copy_(dst)
+    return target
+
+
+def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tensor, kv_indices: torch.Tensor,
+                                           tree_mask: Optional[torch.Tensor] = None, *, q_indptr: torch.Tensor,
+                                           kv_lens: torch.Tensor, kv_indptr: Optional[torch.Tensor] = None,
+                                           kv_layout: str = "NHD", sm_scale: Optional[float] = None,
+                                           out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                                           workspace: Optional[torch.Tensor] = None):
+    """Tree attention over the paged cache, each sequence with its own query and key count.
+
+    q [N, Hq, D], q_indptr, kv_lens and the cache as in append_paged_kv, which
+    writes the query tokens' own keys: token i of sequence b sees the
+    kv_lens[b] - q_len keys before them, and the key of token j of its
+    sequence where tree_mask[b, i, j] (nonzero: visible).  ``tree_mask`` is
+    [B, T, T], or [T, T] for one tree for every sequence; sequences shorter
+    than T use its upper left corner, tokens and columns past T see and are
+    seen by nothing of the tree.  Without a mask token i sees token j <= i
+    (plain decoding at one token, prompts behind a cached prefix).
+
+    O [N, Hq, D] in q's dtype; with ``return_lse`` ``(O, lse)``, lse [N, Hq]
+    float32.  A row that sees no key is 0 (its lse -inf): the uniform forwards
+    return NaN there, as the reference does, but here such rows pad a batch
+    and would carry the NaN into the cache.  Rows behind q_indptr[B] are left
+    as they were.  ``workspace`` (uint8,
+    fwd_paged_varlen_workspace_bytes(...) bytes) must not be shared by calls
+    that overlap in time, captured graphs among them.  No host
+    synchronisation; page ids outside the pool are clamped (wrong O, never an
+    invalid read).
+    """
+    n_pages, page_size, n_kv_heads, head_dim, cache_strides = _paged_pool(kv_cache, kv_layout)
+    if q.dim() != 3 or q.shape[2] != head_dim:
+        raise ValueError(f"q must be [N, Hq, {head_dim}], got {tuple(q.shape)}")
+    n, n_heads = q.shape[0], q.shape[1]
+    if n_kv_heads <= 0 or n_heads % n_kv_heads:
+        raise ValueError("num_heads must be a multiple of the cache's kv heads")
+    if out is not None and tuple(out.shape) != tuple(q.shape):
+        raise ValueError(f"out shape {tuple(out.shape)} != q shape {tuple(q.shape)}")
+    batch, kv_indices, pt_stride, pt_width = _varlen_lists(q_indptr, kv_lens, kv_indices, kv_indptr, page_size)
+    mask = None
+    mask_seq = mask_row = mask_n = 0
+    if tree_mask is not None:
+        if tree_mask.dim() not in (2, 3) or tree_mask.shape[-1] != tree_mask.shape[-2] or tree_mask.shape[-1] < 1:
+            raise ValueError(f"tree_mask must be [T, T] or [{batch}, T, T], got {tuple(tree_mask.shape)}")
+        if tree_mask.dim() == 3 and tree_mask.shape[0] != batch:
+            raise ValueError(f"tree_mask holds {tree_mask.shape[0]} trees for {batch} sequences")
+        mask = tree_mask if tree_mask.dtype == torch.bool else tree_mask != 0
+        if mask.stride(-1) != 1 or min(mask.stride()) < 0:
+            mask = mask.contiguous()
+        mask_n, mask_row = mask.shape[-1], mask.stride(-2)
+        mask_seq = mask.stride(0) if mask.dim() == 3 else 0
+    if q.dtype != kv_cache.dtype or (out is not None and out.dtype != q.dtype):
+        raise NotImplementedError("q, kv_cache and out must share one dtype")
+    dt = _lib.dtype_code(q.dtype)
+    dev = q.device
+    _same_device(dev, q=q, kv_cache=kv_cache, kv_indices=kv_indices, kv_indptr=kv_indptr, q_indptr=q_indptr,
+                 kv_lens=kv_lens, tree_mask=mask, out=out)
+    qc = _row_contig(q)
+    target = torch.empty_like(qc) if out is None else out
+    dst = target if _layout_ok(target) else target.contiguous()
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(head_dim)
+    lib = _lib.load()
+    args = (batch, n, n_heads, n_kv_heads, head_dim, dt)
+    ws_bytes = _varlen_workspace_bytes(dev, args)
+    ws = _workspace(workspace, ws_bytes, dev)
+    lse = torch.empty((n, n_heads), dtype=torch.float32, device=dev) if return_lse else None
+    q_indptr, kv_lens = q_indptr.contiguous(), kv_lens.contiguous()
+    kv_indptr = None if kv_indptr is None else kv_indptr.contiguous()
+    _run_on(dev, "tree_sparse_attention_fwd_paged_varlen", lambda stream: lib.tsfa_fwd_paged_varlen(
+        qc.data_ptr(), kv_cache.data_ptr(), dst.data_ptr(), _lib.ptr(lse), _lib.ptr(mask), mask_seq, mask_row, mask_n,
+        q_indptr.data_ptr(), kv_lens.data_ptr(), _lib.ptr(kv_indptr), kv_indices.data_ptr(),
+        _table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size, _lib.i64_array(qc.stride()),
+        _lib.i64_array(cache_strides), _lib.i64_array(dst.stride()), float(sm_scale), *args, ws.data_ptr(), ws_bytes,
+        stream))
+    if dst is not target:
+        target.copy_(dst)
+    return (target, lse) if return_lse else target
+
+
+def _varlen_workspace_bytes(dev, args) -> int:
+    lib = _lib.load()
+    if dev.index == torch.cuda.current_device():
+        return int(lib.tsfa_fwd_paged_varlen_workspace_bytes(*args))
+    with torch.cuda.device(dev):
+        return int(lib.tsfa_fwd_paged_varlen_workspace_bytes(*args))
+
+
+def fwd_paged_varlen_workspace_bytes(q: torch.Tensor, kv_cache: torch.Tensor, batch: int, *,
+                                     kv_layout: str = "NHD") -> int:
+    """Bytes of the workspace tree_sparse_attention_fwd_paged_varlen uses for this q and ``batch`` sequences
+    (the lengths do not matter)."""
+    _, _, n_kv_heads, head_dim, _ = _paged_pool(kv_cache, kv_layout)
+    return _varlen_workspace_bytes(q.device, (batch, q.shape[0], q.shape[1], n_kv_heads, head_dim,
+                                              _lib.dtype_code(q.dtype)))
+
+
+class BeamSelection(NamedTuple):
+    """What beam_select returns: tokens and parents int64 [B, k], scores float32 [B, k], the reordered states."""
+
+    tokens: torch.Tensor
+    parents: torch.Tensor
+    scores: torch.Tensor
+    states: Tuple[torch.Tensor, ...]
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
+                states: Sequence[torch.Tensor] = ()) -> BeamSelection:
+    """The k best continuations of every sequence over its beams and the vocabulary.
+
+    logits: [B, W, V] float16, bfloat16 or float32 of the W beams; scores:
+        float32 [B, W], the beams' running log-probabilities (W = 1 and a score
+        of 0 at a draft's first step).
+    A continuation's value is (scores[b, w] + logits[b, w, v]) - logsumexp(
+    logits[b, w]), formed and compared in 64 bits; best first, ties to the
+    lowest w * V + v.  NaN logits count as -inf, and a -inf logit is no
+    continuation; a beam whose score is not finite has none.  Slots past the
+    last continuation hold token 0, parent 0 and score -inf, so the next step
+    ignores them.
+    states: tensors [B, W, ...] (hidden states, page tables, tree rows) of any
+        dtype; the result holds states[i][b, parents[b]] as [B, k, ...].
+    A draft's tree grows by ``parents``: continuation j of this step is a child
+    of continuation parents[b, j] of the step before.
+    """
+    if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]):
+        raise ValueError(f"logits must be [B, W, V] and scores [B, W], got {tuple(logits.shape)} and "
+                         f"{tuple(scores.shape)}")
+    if scores.dtype != torch.float32:
+        raise ValueError("scores must be float32")
+    batch, beams, vocab = logits.shape
+    if beams < 1 or vocab < 1 or k < 1 or k > beams * vocab:
+        raise ValueError(f"k must be between 1 and W * V, got {k} of {beams} * {vocab}")
+    dt = _lib.dtype_code(logits.dtype)
+    dev = logits.device
+    _same_device(dev, logits=logits, scores=scores)
+    for i, t in enumerate(states):
+        if t.dim() < 2 or tuple(t.shape[:2]) != (batch, beams):
+            raise ValueError(f"states[{i}] must be [{batch}, {beams}, ...], got {tuple(t.shape)}")
+        _same_device(dev, **{f"states[{i}]": t})
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
+    lib = _lib.load()
+    new = dict(device=dev, dtype=torch.int64)
+    tokens, parents = torch.empty((batch, k), **new), torch.empty((batch, k), **new)
+    best = torch.empty((batch, k), dtype=torch.float32, device=dev)
+    src = [t.contiguous() for t in states]
+    dst = [torch.empty((batch, k, *t.shape[2:]), dtype=t.dtype, device=dev) for t in src]
+    n = len(src)
+    pointers = ctypes.c_void_p * max(n, 1)
+    row_bytes = [t[0, 0].numel() * t.element_size() if t.numel() else 0 for t in src]
+    ws_bytes = int(lib.tsfa_beam_select_workspace_bytes(batch, beams, vocab, k))
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=dev)
+    _run_on(dev, "beam_select", lambda stream: lib.tsfa_beam_select(
+        logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), scores.stride(0), scores.stride(1),
+        batch, beams, vocab, k, dt, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(),
+        pointers(*(t.data_ptr() for t in src)), pointers(*(t.data_ptr() for t in dst)), _lib.i64_array(row_bytes), n,
+        ws.data_ptr(), ws_bytes, stream))
+    return BeamSelection(tokens, parents, best, tuple(dst))

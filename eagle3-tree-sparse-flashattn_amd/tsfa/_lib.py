@@ -51,6 +51,11 @@ EXPORTS = (
     "tsfa_bwd",
     "tsfa_bwd_workspace_bytes",
     "tsfa_fwd_paged",
+    "tsfa_append_paged_kv",
+    "tsfa_fwd_paged_varlen",
+    "tsfa_fwd_paged_varlen_workspace_bytes",
+    "tsfa_beam_select",
+    "tsfa_beam_select_workspace_bytes",
     "tsfa_fwd_plan",
     "tsfa_fwd_set_kernel_mask",
 )
@@ -91,6 +96,16 @@ _SIGNATURES = {
     "tsfa_fwd_paged": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_int, _c_int, _c_vp, _c_vp,
                                 _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]
                        + [ctypes.POINTER(_c_i64)] * 4 + [_c_float] + [_c_int] * 13 + [_c_vp, _c_size, _c_vp]),
+    "tsfa_append_paged_kv": (_c_int, [_c_vp] * 6 + [_c_int, _c_vp, _c_int, _c_int, _c_float] + [_c_vp] * 4
+                             + [_c_i64, _c_i64, _c_int, _c_int, _c_int] + [ctypes.POINTER(_c_i64)] * 2
+                             + [_c_int] * 6 + [_c_vp]),
+    "tsfa_fwd_paged_varlen_workspace_bytes": (_c_size, [_c_int] * 6),
+    "tsfa_fwd_paged_varlen": (_c_int, [_c_vp] * 5 + [_c_i64, _c_i64, _c_int] + [_c_vp] * 4
+                              + [_c_i64, _c_i64, _c_int, _c_int, _c_int] + [ctypes.POINTER(_c_i64)] * 3 + [_c_float]
+                              + [_c_int] * 6 + [_c_vp, _c_size, _c_vp]),
+    "tsfa_beam_select_workspace_bytes": (_c_size, [_c_int] * 4),
+    "tsfa_beam_select": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64] + [_c_int] * 5 + [_c_vp] * 3
+                         + [ctypes.POINTER(_c_vp)] * 2 + [ctypes.POINTER(_c_i64), _c_int, _c_vp, _c_size, _c_vp]),
     "tsfa_fwd_plan": (_c_int, [_c_int] * 7 + [ctypes.POINTER(ctypes.c_int32)]),
     "tsfa_fwd_set_kernel_mask": (_c_int, [_c_int]),
 }

@@ -229,6 +229,97 @@ int tsfa_fwd_paged(const void* q, const void* kv_cache, const int32_t* kv_indptr
                    int block_m, int block_n, int head_dim, int dtype,
                    void* workspace, size_t workspace_bytes, tsfa_stream_t stream);
 
+/* ------------------------------------------- serving over the paged cache
+ * Drafted tokens of a batch whose sequences have different lengths, all of
+ * them on the device: no host synchronisation, and a captured graph follows
+ * the lengths.  No counterpart in the reference.  Shared arguments:
+ *
+ * q_indptr       int32[batch + 1]: the query tokens of sequence b are rows
+ *                [q_indptr[b], q_indptr[b + 1]) of the packed [total_q, H, D]
+ *                tensors; rows at or behind q_indptr[batch] belong to no
+ *                sequence and are neither read nor written
+ * kv_lens        int32[batch]: keys of each sequence with its query tokens'
+ *                own (query token i is key kv_lens[b] - q_len + i)
+ * kv_indptr, kv_indices, n_indices, page_table_stride, n_pages, page_size,
+ * cache_strides  the pool and the page lists as in tsfa_fwd_paged, with lists
+ *                of their own lengths: kv_indices[kv_indptr[b] ..
+ *                kv_indptr[b + 1]), or page_table_width entries at
+ *                kv_indices[b * page_table_stride]
+ * Device values out of range address nothing: lengths are cut to what the
+ * list's pages and total_q hold, page ids clamped (attention) or skipped
+ * (append).
+ *
+ * tsfa_append_paged_kv rotates q into out and k into the pool, and copies v:
+ * pair i of the first rot_dim elements of a head, (i, rot_dim / 2 + i) or,
+ * interleaved, (2i, 2i + 1), is turned by positions[n] * inv_freq[i] and
+ * multiplied by attention_scaling; the other elements are copied.
+ * q, out     [total_q, num_heads, head_dim] (out may be q)
+ * k, v       [total_q, num_kv_heads, head_dim]
+ * positions  int64 (positions_64 != 0) or int32 [total_q]
+ * inv_freq   fp32 [rot_dim / 2]; the angle is formed in 64 bits
+ * strides    int64[12]: q, k, v, out -- (token, head, d) each, in elements;
+ *            d strides 1, rows 16-byte aligned
+ * Supported: fp16 / bf16; head_dim <= 256 and rot_dim <= head_dim, multiples
+ * of 16.  Two tokens must not share a place in the pool. */
+int tsfa_append_paged_kv(const void* q, const void* k, const void* v, void* out, void* kv_cache,
+                         const void* positions, int positions_64, const float* inv_freq, int rot_dim,
+                         int interleaved, float attention_scaling, const int32_t* q_indptr,
+                         const int32_t* kv_lens, const int32_t* kv_indptr, const int32_t* kv_indices,
+                         int64_t n_indices, int64_t page_table_stride, int page_table_width, int n_pages,
+                         int page_size, const int64_t* strides, const int64_t* cache_strides, int batch,
+                         int total_q, int num_heads, int num_kv_heads, int head_dim, int dtype,
+                         tsfa_stream_t stream);
+
+/* Tree attention of those tokens: token i of a sequence sees its
+ * kv_lens - q_len prefix keys, and the key of token j iff mask[b][i][j] != 0
+ * (mask NULL: iff j <= i).  O [total_q, num_heads, head_dim] in the input
+ * dtype, one rounding of the fp32 result; a row that sees no key is 0 (its
+ * LSE -inf), so that rows that pad a batch carry no NaN into the next layer's
+ * keys.  Infinities and NaN of keys a row does not see do not reach it.
+ * mask       uint8, element (b, i, j) at b * mask_seq_stride + i *
+ *            mask_row_stride + j, mask_n rows and columns (0 stride: one tree
+ *            for the batch); tokens and columns past mask_n are not visible
+ * lse        NULL, or fp32 [total_q, num_heads]: log sum exp of the scaled
+ *            visible scores
+ * q_strides, o_strides  int64[3]: token, head, d
+ * workspace  tsfa_fwd_paged_varlen_workspace_bytes, 16-byte aligned; its size
+ *            does not depend on the lengths
+ * Supported: fp16 / bf16, head_dim 64 or 128, num_heads a multiple of
+ * num_kv_heads (at most 256 times), up to 2^30 keys per sequence. */
+size_t tsfa_fwd_paged_varlen_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads, int head_dim,
+                                             int dtype);
+int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* o, float* lse, const uint8_t* mask,
+                          int64_t mask_seq_stride, int64_t mask_row_stride, int mask_n,
+                          const int32_t* q_indptr, const int32_t* kv_lens, const int32_t* kv_indptr,
+                          const int32_t* kv_indices, int64_t n_indices, int64_t page_table_stride,
+                          int page_table_width, int n_pages, int page_size, const int64_t* q_strides,
+                          const int64_t* cache_strides, const int64_t* o_strides, float sm_scale, int batch,
+                          int total_q, int num_heads, int num_kv_heads, int head_dim, int dtype,
+                          void* workspace, size_t workspace_bytes, tsfa_stream_t stream);
+
+/* One step of a draft or beam search: the k best continuations of every
+ * sequence over its beams and the vocabulary, and the beams' states in the
+ * order of the selected parents.
+ *   value(w, v) = (scores[b][w] + logits[b][w][v]) - log sum_v' exp(logits[b][w][v'])
+ * in 64 bits, best first, ties to the lowest w * vocab + v.  NaN logits count
+ * as -inf, which is no candidate; a beam whose score is not finite has none
+ * (tokens at +inf share their beam's mass).  Slots past the last candidate
+ * hold token 0, parent 0, score -inf.
+ * logits     [batch, beams, vocab] of `dtype` (fp16, bf16 or fp32), vocab
+ *            stride 1; scores fp32; strides in elements
+ * tokens, parents int64 [batch, k]; out_scores fp32 [batch, k]
+ * states     n_states (at most 8) host pointers to [batch, beams] dense rows
+ *            of state_row_bytes bytes, copied to out_states [batch, k]
+ * Supported: k <= 64 (and <= beams * vocab), beams <= 256, beams * vocab <=
+ * 2^30, batch * k <= 65535.  workspace 16-byte aligned. */
+size_t tsfa_beam_select_workspace_bytes(int batch, int beams, int vocab, int k);
+int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, int64_t logits_beam_stride,
+                     const float* scores, int64_t scores_seq_stride, int64_t scores_beam_stride, int batch,
+                     int beams, int vocab, int k, int dtype, int64_t* tokens, int64_t* parents,
+                     float* out_scores, const void* const* states, void* const* out_states,
+                     const int64_t* state_row_bytes, int n_states, void* workspace, size_t workspace_bytes,
+                     tsfa_stream_t stream);
+
 /* run_tree_sparse_kernel(q, k, v, tree_mask) in one call
  * (eagle_tree_sparse_bridge.py:76-159: metadata from the tree mask, then the
  * forward with prefix_len = kv_len - q_len, eagle_tree_sparse_bridge.py:91-117):
