@@ -27,6 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxK = 64;
 constexpr int kMaxBeams = 256;
 constexpr int kMaxStates = 8;
+constexpr int64_t kStatesInside = 256 << 10;
 
 // Statistics of one tile: maximum (as a float) and sum of exp(x - maximum).
 struct PartStat {
@@ -58,21 +59,62 @@ __device__ inline float key_logit(uint64_t key) {
 }
 __device__ inline uint32_t key_token(uint64_t key) { return ~(uint32_t)key; }
 
-// exp(x - top) for x <= top, with exp(0) also for equal infinities.
-__device__ inline double weight(float x, float top) {
-  if (x == top) return 1.0;
-  return exp((double)x - (double)top);
+// 2^(x log2 e) for x <= 0 (below -700: the value at -700, which no sum of
+// such weights notices): x log2 e = n + f, 2^f by the polynomial of degree 9
+// through the Chebyshev points of [-1/2, 1/2] (2e-14 off at most), n into the
+// exponent.  Adding 1.5 * 2^52 rounds to n and leaves it in the low word.
+__device__ inline double exp_neg(double x) {
+  constexpr double kRound = 6755399441055744.0;
+  const double t = fmax(x, -700.0) * 1.4426950408889634074;
+  const double u = t + kRound;
+  const double f = t - (u - kRound);
+  double p = 1.0205905413765595e-07;
+  p = fma(p, f, 1.325964524488711e-06);
+  p = fma(p, f, 1.5252672924850737e-05);
+  p = fma(p, f, 0.0001540343375125101);
+  p = fma(p, f, 0.0013333558200794592);
+  p = fma(p, f, 0.009618129193934313);
+  p = fma(p, f, 0.05550410866465167);
+  p = fma(p, f, 0.2402265069564034);
+  p = fma(p, f, 0.6931471805599462);
+  p = fma(p, f, 1.0000000000000135);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, u) << 52);
+  return __builtin_bit_cast(double, bits);
+}
+// exp(x - top) for x <= top, top > -inf; equal infinities weigh 1.
+__device__ inline double weight(float x, float top) { return x == top ? 1.0 : exp_neg((double)x - (double)top); }
+
+// The largest v that at least k of the wave's keys a and b are not below, from
+// the top bit down by counting lanes; 1 if fewer than k are not 0.  Keys of
+// distinct candidates differ, so exactly k keys reach it.
+__device__ inline uint64_t kth_key(uint64_t a, uint64_t b, int k) {
+  auto count = [](bool x, bool y) { return __builtin_popcountll(__ballot(x)) + __builtin_popcountll(__ballot(y)); };
+  if (count(a != 0, b != 0) < k) return 1;
+  const uint32_t ah = (uint32_t)(a >> 32), bh = (uint32_t)(b >> 32);
+  uint32_t hi = 0;
+  for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
+    const int c = count(ah >= (hi | bit), bh >= (hi | bit));
+    if (c >= k) hi |= bit;
+    if (c == k) return (uint64_t)hi << 32;
+  }
+  const int above = count(ah > hi, bh > hi);
+  uint32_t lo = 0;
+  for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
+    const int c = above + count(ah == hi && (uint32_t)a >= (lo | bit), bh == hi && (uint32_t)b >= (lo | bit));
+    if (c >= k) lo |= bit;
+    if (c == k) break;
+  }
+  return ((uint64_t)hi << 32) | lo;
 }
 
 // EPT elements per thread, VEC of them in one 16-byte load.
 template <typename T, int EPT>
 __global__ __launch_bounds__(kThreads) void part_kernel(const PartArgs a) {
-  constexpr int VEC = 16 / (int)sizeof(T), NU = EPT / VEC;
-  __shared__ __attribute__((aligned(16))) uint64_t best[kThreads];
-  __shared__ uint64_t list[kMaxK * EPT];
-  __shared__ double wsum[kThreads / 64];
-  __shared__ float wtop[kThreads / 64];
-  __shared__ uint64_t bound;
+  constexpr int VEC = 16 / (int)sizeof(T), NU = EPT / VEC, NW = kThreads / 64, H = EPT / 2;
+  __shared__ __attribute__((aligned(16))) uint64_t list[2 * kMaxK * EPT];
+  __shared__ double wsum[NW];
+  __shared__ float wtop[NW];
+  __shared__ uint64_t wbound[NW];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tile = blockIdx.x % a.tiles, row = blockIdx.x / a.tiles;
@@ -95,61 +137,73 @@ __global__ __launch_bounds__(kThreads) void part_kernel(const PartArgs a) {
     }
   }
   auto token = [&](int e) { return (uint32_t)(v0 + ((e / VEC) * kThreads + tid) * VEC + e % VEC); };
+  if (tid == 0) count = 0;
 
-  if (tid == 0) {
-    bound = 1;  // fewer than k threads hold a candidate: all of them
-    count = 0;
-  }
-  float top = -INFINITY;
-  uint64_t mine = 0;
+  // the best of each half of the thread's elements (the lowest token of equal
+  // ones: tokens rise with e)
+  float fa = -INFINITY, fb = -INFINITY;
 #pragma unroll
   for (int e = 0; e < EPT; ++e) {
     if (!(xs[e] == xs[e])) xs[e] = -INFINITY;  // NaN is no candidate and weighs nothing
-    top = fmaxf(top, xs[e]);
-    const uint64_t key = make_key(xs[e], token(e));
-    mine = key > mine ? key : mine;
+    if (e < H) fa = fmaxf(fa, xs[e]);
+    else fb = fmaxf(fb, xs[e]);
   }
-  best[tid] = mine;
+  int ea = 0, eb = H;
+#pragma unroll
+  for (int e = H - 1; e >= 0; --e) {
+    if (xs[e] == fa) ea = e;
+    if (xs[e + H] == fb) eb = e + H;
+  }
+  const uint64_t ka = make_key(fa, token(ea)), kb = make_key(fb, token(eb));
+  float top = fmaxf(fa, fb);
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
-  if (lane == 0) wtop[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) top = fmaxf(top, wtop[i]);
-
-  double sum = 0;
-  if (top > -INFINITY) {
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) sum += weight(xs[e], top);
-  }
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-  if (lane == 0) wsum[wave] = sum;
-
-  // The k-th best of the threads' best bounds the tile's k-th best from below,
-  // and only the k threads at or above it hold anything better: at most k *
-  // EPT elements whatever the values are.
-  if (mine != 0) {
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < kThreads; ++i) rank += best[i] > mine;
-    if (rank == a.k - 1) bound = mine;
+  // Each wave's k-th best half bounds the tile's k-th best element from below,
+  // the best of these bounds closest; at most k halves of every wave reach it,
+  // 2 k EPT elements whatever the values are (a few times k for a model's).
+  const uint64_t wb = kth_key(ka, kb, a.k);
+  if (lane == 0) {
+    wtop[wave] = top;
+    wbound[wave] = wb;
   }
   __syncthreads();
-  const uint64_t lim = bound;
-  if (mine >= lim) {
+  uint64_t lim = 1;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    top = fmaxf(top, wtop[i]);
+    lim = wbound[i] > lim ? wbound[i] : lim;
+  }
+  if (ka >= lim || kb >= lim) {
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
       const uint64_t key = make_key(xs[e], token(e));
       if (key >= lim) list[atomicAdd(&count, 1)] = key;
     }
   }
+
+  double sum = 0, sum2 = 0;
+  if (top == INFINITY) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) sum += xs[e] == top ? 1.0 : 0.0;
+  } else if (top > -INFINITY) {
+    const double t = top;
+#pragma unroll
+    for (int e = 0; e < EPT; e += 2) {
+      sum += exp_neg((double)xs[e] - t);
+      sum2 += exp_neg((double)xs[e + 1] - t);
+    }
+    sum += sum2;
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+  if (lane == 0) wsum[wave] = sum;
   __syncthreads();
   const int n = count;
   uint64_t* out = a.keys + ((int64_t)row * a.tiles + tile) * a.k;
   for (int i = tid; i < n; i += kThreads) {
     const uint64_t key = list[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += list[j] > key;
     if (rank < a.k) out[rank] = key;
   }
@@ -158,10 +212,30 @@ __global__ __launch_bounds__(kThreads) void part_kernel(const PartArgs a) {
     PartStat st;
     st.sum = 0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) st.sum += wsum[i];
+    for (int i = 0; i < NW; ++i) st.sum += wsum[i];
     st.top = top;
     st.pad = 0;
     a.stats[(int64_t)row * a.tiles + tile] = st;
+  }
+}
+
+// The states' rows of the parents, [batch][beams] to [batch][k].
+struct States {
+  const void* src[kMaxStates];
+  void* dst[kMaxStates];
+  int64_t row_bytes[kMaxStates];
+  int n;
+};
+// Threads first, first + step, ... copy one row.
+__device__ inline void copy_row(const States& st, int s, int64_t from, int64_t to, int64_t first, int64_t step) {
+  const int64_t bytes = st.row_bytes[s];
+  const char* src = static_cast<const char*>(st.src[s]) + from * bytes;
+  char* dst = static_cast<char*>(st.dst[s]) + to * bytes;
+  if (((reinterpret_cast<uintptr_t>(st.src[s]) | reinterpret_cast<uintptr_t>(st.dst[s]) | (uintptr_t)bytes) & 15) == 0) {
+    for (int64_t i = first; i < bytes / 16; i += step)
+      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+  } else {
+    for (int64_t i = first; i < bytes; i += step) dst[i] = src[i];
   }
 }
 
@@ -174,45 +248,61 @@ struct MergeArgs {
   int64_t* tokens;
   int64_t* parents;
   float* out_scores;
+  States states;  // n = 0: copied by states_kernel
 };
 
-// A candidate over all beams: value, then the lower w * vocab + v.  None: -inf.
+// A candidate over all beams, better = larger value, then the lower flat = w *
+// vocab + v.  The value is a double in an order of its bits that integers
+// compare alike; 0 is no candidate.
 struct Cand {
-  double value;
+  uint64_t value;
   uint32_t flat, pad;
 };
 __device__ inline bool better(const Cand& x, const Cand& y) {
   return x.value > y.value || (x.value == y.value && x.flat < y.flat);
 }
+__device__ inline uint64_t value_key(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
+  return u >> 63 ? ~u : u | ((uint64_t)1 << 63);
+}
+__device__ inline double key_value(uint64_t o) {
+  return __builtin_bit_cast(double, o >> 63 ? o & ~((uint64_t)1 << 63) : ~o);
+}
 
-constexpr int kBatch = 4;  // candidates per thread and round
+constexpr int kMergeThreads = 512;
+constexpr int kBatch = 8;     // candidates per thread and round
+constexpr int kMergeList = 1024;
 
-__global__ __launch_bounds__(kThreads) void merge_kernel(const MergeArgs a) {
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a) {
+  constexpr int NW = kMergeThreads / 64;
+  static_assert(kMergeList >= kMaxK * kBatch + kMaxK, "a round's candidates by rank");
   __shared__ double lse[kMaxBeams], score[kMaxBeams];
   __shared__ float tops[kMaxBeams];
-  __shared__ Cand heads[kThreads];
-  __shared__ Cand list[kMaxK * kBatch + kMaxK];
+  __shared__ Cand heads[kMergeThreads];
+  __shared__ Cand list[kMergeList];
   __shared__ Cand kept[kMaxK];
+  __shared__ uint64_t wbound[NW];
   __shared__ Cand bound;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x;
-  const Cand none = {-INFINITY, 0xffffffffu, 0};
+  const Cand none = {0, 0xffffffffu, 0};
 
-  // lse_w = top + log(sum) of the tiles; a beam with no finite or infinite
-  // logit, or whose score is not finite, has no candidates
-  for (int w = wave; w < a.beams; w += kThreads / 64) {
-    const PartStat* st = a.stats + ((int64_t)b * a.beams + w) * a.tiles;
+  // lse_w = top + log(sum) of the tiles, 16 lanes to a beam; a beam with
+  // nothing above -inf, or whose score is not finite, has no candidates
+  for (int w0 = 0; w0 < a.beams; w0 += kMergeThreads / 16) {
+    const int w = w0 + tid / 16, l = tid & 15;
+    const PartStat* st = a.stats + ((int64_t)b * a.beams + (w < a.beams ? w : a.beams - 1)) * a.tiles;
     float top = -INFINITY;
-    for (int i = lane; i < a.tiles; i += 64) top = fmaxf(top, st[i].top);
+    for (int i = l; i < a.tiles; i += 16) top = fmaxf(top, st[i].top);
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+    for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
     double sum = 0;
-    for (int i = lane; i < a.tiles; i += 64)
+    for (int i = l; i < a.tiles; i += 16)
       if (st[i].top > -INFINITY) sum += st[i].sum * weight(st[i].top, top);
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-    if (lane == 0) {
+    for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+    if (l == 0 && w < a.beams) {
       const float c = a.scores[b * a.ssb + w * a.ssw];
       const bool alive = top > -INFINITY && c - c == 0.0f;
       tops[w] = top;
@@ -222,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const MergeArgs a) {
       lse[w] = top < INFINITY ? (double)top + log(sum) : log(sum);
     }
   }
-  for (int i = tid; i < a.k; i += kThreads) kept[i] = none;
+  for (int i = tid; i < a.k; i += kMergeThreads) kept[i] = none;
   __syncthreads();
 
   // Candidates in rounds, the tiles' best first, so that the first rounds
@@ -230,22 +320,22 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const MergeArgs a) {
   const int lists = a.beams * a.tiles;
   const int64_t total = (int64_t)lists * a.k;
   const uint64_t* keys = a.keys + (int64_t)b * lists * a.k;
-  for (int64_t c0 = 0; c0 < total; c0 += kThreads * kBatch) {
+  for (int64_t c0 = 0; c0 < total; c0 += kMergeThreads * kBatch) {
     const Cand last = kept[a.k - 1];
     Cand cs[kBatch], top = none;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int64_t c = c0 + j * kThreads + tid;
+      const int64_t c = c0 + j * kMergeThreads + tid;
       cs[j] = none;
       if (c < total) {
-        const int p = (int)(c / lists), l = (int)(c - (int64_t)p * lists);
+        const int p = (int)((uint32_t)c / (uint32_t)lists), l = (int)((uint32_t)c - (uint32_t)p * (uint32_t)lists);
         const uint64_t key = keys[(int64_t)l * a.k + p];
         const int w = l / a.tiles;
         if (key != 0 && score[w] > -INFINITY) {
           const float x = key_logit(key);
           const bool inf = tops[w] == INFINITY;
           if (!inf || x == INFINITY) {
-            cs[j].value = (score[w] + (inf ? 0.0 : (double)x)) - lse[w];
+            cs[j].value = value_key((score[w] + (inf ? 0.0 : (double)x)) - lse[w]);
             cs[j].flat = (uint32_t)w * (uint32_t)a.vocab + key_token(key);
           }
         }
@@ -253,67 +343,80 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const MergeArgs a) {
       if (!better(cs[j], last)) cs[j] = none;
       if (better(cs[j], top)) top = cs[j];
     }
-    heads[tid] = top;
-    if (tid == 0) {
-      bound = last;
-      count = 0;
-    }
-    if (__syncthreads_or(top.value > -INFINITY) == 0) continue;
-    if (top.value > -INFINITY) {
-      int rank = 0;
-#pragma unroll 4
-      for (int i = 0; i < kThreads; ++i) rank += better(heads[i], top);
-      if (rank == a.k - 1) bound = top;  // k candidates at least as good
-    }
+    if (tid == 0) count = 0;
+    if (__syncthreads_or(top.value != 0) == 0) continue;
+    // as in part_kernel, by value alone: ties at the bound stay in
+    const uint64_t wb = kth_key(top.value, 0, a.k);
+    if (lane == 0) wbound[wave] = wb;
     __syncthreads();
-    const Cand lim = bound;
+    uint64_t lim = last.value > 1 ? last.value : 1;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) lim = wbound[i] > lim ? wbound[i] : lim;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
-      if (cs[j].value > -INFINITY && !better(lim, cs[j])) list[atomicAdd(&count, 1)] = cs[j];
+      if (cs[j].value >= lim) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kMergeList - kMaxK) list[at] = cs[j];
+      }
     __syncthreads();
-    const int n = count;
+    int n = count;
+    if (n > kMergeList - kMaxK) {
+      // more ties than the list holds: the k-th best thread by value and
+      // place, which at most k threads reach
+      heads[tid] = top;
+      if (tid == 0) {
+        bound = last;
+        count = 0;
+      }
+      __syncthreads();
+      if (top.value != 0) {
+        int rank = 0;
+        for (int i = 0; i < kMergeThreads; ++i) rank += better(heads[i], top);
+        if (rank == a.k - 1) bound = top;
+      }
+      __syncthreads();
+      const Cand by = bound;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (cs[j].value != 0 && !better(by, cs[j])) list[atomicAdd(&count, 1)] = cs[j];
+      __syncthreads();
+      n = count;
+    }
     // the kept ones join, all are ranked, the k best stay
-    for (int i = tid; i < a.k; i += kThreads) list[n + i] = kept[i];
+    for (int i = tid; i < a.k; i += kMergeThreads) list[n + i] = kept[i];
     __syncthreads();
-    for (int i = tid; i < n + a.k; i += kThreads) {
+    for (int i = tid; i < n + a.k; i += kMergeThreads) {
       const Cand x = list[i];
-      if (x.value == -INFINITY) continue;
+      if (x.value == 0) continue;
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n + a.k; ++j) rank += better(list[j], x);
       if (rank < a.k) kept[rank] = x;
     }
     __syncthreads();
   }
-  for (int i = tid; i < a.k; i += kThreads) {
+  for (int i = tid; i < a.k; i += kMergeThreads) {
     const Cand x = kept[i];
-    const bool ok = x.value > -INFINITY;
+    const bool ok = x.value != 0;
     const int64_t at = (int64_t)b * a.k + i;
-    a.tokens[at] = ok ? (int64_t)(x.flat % (uint32_t)a.vocab) : 0;
-    a.parents[at] = ok ? (int64_t)(x.flat / (uint32_t)a.vocab) : 0;
-    a.out_scores[at] = ok ? (float)x.value : -INFINITY;
+    const uint32_t w = ok ? x.flat / (uint32_t)a.vocab : 0;
+    a.tokens[at] = ok ? (int64_t)(x.flat - w * (uint32_t)a.vocab) : 0;
+    a.parents[at] = (int64_t)w;
+    a.out_scores[at] = ok ? (float)key_value(x.value) : -INFINITY;
+    kept[i].pad = w;
   }
+  if (a.states.n == 0) return;
+  __syncthreads();
+  for (int s = 0; s < a.states.n; ++s)
+    for (int i = wave; i < a.k; i += NW)
+      copy_row(a.states, s, (int64_t)b * a.beams + kept[i].pad, (int64_t)b * a.k + i, lane, 64);
 }
 
-struct StatesArgs {
-  const void* src[kMaxStates];
-  void* dst[kMaxStates];
-  int64_t row_bytes[kMaxStates];
-  const int64_t* parents;  // [batch][k]
-  int beams, k;
-};
-
-__global__ __launch_bounds__(kThreads) void states_kernel(const StatesArgs a) {
-  const int s = blockIdx.z, at = blockIdx.y;
-  const int64_t bytes = a.row_bytes[s];
-  const char* src = static_cast<const char*>(a.src[s]) + ((int64_t)(at / a.k) * a.beams + a.parents[at]) * bytes;
-  char* dst = static_cast<char*>(a.dst[s]) + (int64_t)at * bytes;
-  const int64_t i0 = (int64_t)blockIdx.x * kThreads + threadIdx.x, step = (int64_t)gridDim.x * kThreads;
-  if (((reinterpret_cast<uintptr_t>(a.src[s]) | reinterpret_cast<uintptr_t>(a.dst[s]) | (uintptr_t)bytes) & 15) == 0) {
-    for (int64_t i = i0; i < bytes / 16; i += step)
-      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-  } else {
-    for (int64_t i = i0; i < bytes; i += step) dst[i] = src[i];
-  }
+// States too large for the merge's one workgroup per sequence.
+__global__ __launch_bounds__(kThreads) void states_kernel(const States st, const int64_t* parents, int beams, int k) {
+  const int at = blockIdx.y;
+  copy_row(st, blockIdx.z, (int64_t)(at / k) * beams + parents[at], at, (int64_t)blockIdx.x * kThreads + threadIdx.x,
+           (int64_t)gridDim.x * kThreads);
 }
 
 // Elements of a tile per thread: long tiles where the rows alone fill the
@@ -368,8 +471,8 @@ extern "C" int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, i
   if (batch == 0) return TSFA_OK;
   if (logits == nullptr || scores == nullptr || tokens == nullptr || parents == nullptr || out_scores == nullptr)
     return TSFA_ERR_INVALID_ARGUMENT;
-  StatesArgs sa;
-  int64_t most = 0;
+  States sa;
+  int64_t most = 0, moved = 0;
   for (int i = 0; i < n_states; ++i) {
     if (states == nullptr || out_states == nullptr || state_row_bytes == nullptr || state_row_bytes[i] < 0)
       return TSFA_ERR_INVALID_ARGUMENT;
@@ -378,6 +481,7 @@ extern "C" int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, i
     sa.dst[i] = out_states[i];
     sa.row_bytes[i] = state_row_bytes[i];
     most = state_row_bytes[i] > most ? state_row_bytes[i] : most;
+    moved += state_row_bytes[i];
   }
   const int64_t rows = (int64_t)batch * beams;
   const int ept = elements_per_thread(rows, vocab);
@@ -415,15 +519,17 @@ extern "C" int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, i
   ma.tokens = tokens;
   ma.parents = parents;
   ma.out_scores = out_scores;
-  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)batch), dim3(kThreads), 0, s, ma);
-
-  if (most > 0) {
-    sa.parents = parents;
-    sa.beams = beams;
-    sa.k = k;
+  // The merge's workgroup copies a sequence's states itself where they are
+  // small enough that a launch for them costs more.
+  sa.n = n_states;
+  const bool inside = moved * k <= kStatesInside;
+  ma.states = sa;
+  if (!inside) ma.states.n = 0;
+  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)batch), dim3(kMergeThreads), 0, s, ma);
+  if (!inside) {
     const int64_t blocks = (most / 16 + kThreads) / kThreads;
     hipLaunchKernelGGL(states_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), (unsigned)(batch * k), (unsigned)n_states),
-                       dim3(kThreads), 0, s, sa);
+                       dim3(kThreads), 0, s, sa, (const int64_t*)parents, beams, k);
   }
   return hipGetLastError() == hipSuccess ? TSFA_OK : TSFA_ERR_LAUNCH;
 }

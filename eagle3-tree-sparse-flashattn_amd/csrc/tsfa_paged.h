@@ -58,66 +58,137 @@ TSFA_HD inline Seq seq_of(const Seqs& s, int b) {
 // ---------------------------------------------------- the attention's work
 // The query rows of one (sequence, kv head) are packed token-major, r = t *
 // group + g, and cut into tiles of `rows`; a tile walks its keys in steps of
-// `keys`.  All steps of a call, in the order (sequence, kv head, tile, step),
-// form one line that is cut into equal runs, one to a workgroup: every
-// workgroup gets the same number of steps whatever the lengths are, and at
-// most the first and the last tile of a run are shared with its neighbours.
+// `keys`.  All tiles of a call lie on one line in the order (sequence, kv
+// head, tile), each as long as its keys, and the line is cut into equal runs,
+// one to a workgroup: the run of a step is the one its start lies in, so every
+// workgroup gets about the same work whatever the lengths are and at most the
+// first and the last tile of a run are shared with its neighbours.
+//
+// The line counts 1 / group keys, step s of a tile starting s * unit past the
+// tile.  With a mask every tile of a sequence sees its kv_len keys and is a
+// whole number of steps long.  Without, tile r ends at its last token's own
+// key, prefix + ((r + 1) rows - 1) / group, linear in r on this scale, so the
+// place of a tile is a closed form both ways and no workgroup walks the tiles
+// before its own (a loop over them took tens of microseconds for prompts of
+// 1000 tokens).  Either way steps start a step's length apart at least.
 struct Cut {
-  int rows, keys;           // tile height, keys of a step
+  int rows, keys;           // tile height, keys of a step (powers of two)
   int group, num_kv_heads;  // query heads per kv head; kv heads
   int causal;               // no mask: a tile stops at its last token's own key
+  int keys_shift, rows_shift;
+  FastDiv by_group;
+  int64_t unit;             // line length of a step: keys * group
+  double inv_unit;
 };
 
+inline Cut make_cut(int rows, int keys, int group, int num_kv_heads, int causal) {
+  Cut c;
+  c.rows = rows;
+  c.keys = keys;
+  c.group = group;
+  c.num_kv_heads = num_kv_heads;
+  c.causal = causal;
+  for (c.keys_shift = 0; (1 << c.keys_shift) < keys;) ++c.keys_shift;
+  for (c.rows_shift = 0; (1 << c.rows_shift) < rows;) ++c.rows_shift;
+  c.by_group = make_fastdiv((uint32_t)group);
+  c.unit = (int64_t)keys * group;
+  c.inv_unit = 1.0 / (double)c.unit;
+  return c;
+}
+
+// x / d for 0 <= x < 2^52, inv = 1 / d: off by one at most before the remainder is looked at.
+TSFA_HD inline int64_t udiv(int64_t x, int64_t d, double inv) {
+  int64_t q = (int64_t)((double)x * inv);
+  const int64_t r = x - q * d;
+  if (r < 0) --q;
+  else if (r >= d) ++q;
+  return q;
+}
+
 TSFA_HD inline int cut_tiles(const Cut& c, const Seq& s) {
-  return (int)(((int64_t)s.q_len * c.group + c.rows - 1) / c.rows);
+  return (int)(((int64_t)s.q_len * c.group + c.rows - 1) >> c.rows_shift);
 }
 
 // Steps of tile r (at least one: a tile without keys still writes its rows).
 TSFA_HD inline int tile_steps(const Cut& c, const Seq& s, int r) {
   int end = s.kv_len;
   if (c.causal) {
-    const int64_t t = (((int64_t)r + 1) * c.rows - 1) / c.group;  // the tile's last token
-    const int64_t lim = (int64_t)s.prefix + (t < s.q_len ? t + 1 : s.q_len);
-    if (lim < end) end = (int)lim;
+    const int t = (int)fdiv(((uint32_t)r + 1) * (uint32_t)c.rows - 1, c.by_group);  // the tile's last token
+    const int lim = s.prefix + (t < s.q_len ? t + 1 : s.q_len);
+    if (lim < end) end = lim;
   }
-  const int n = (int)(((int64_t)end + c.keys - 1) / c.keys);
+  const int n = (int)(((int64_t)end + c.keys - 1) >> c.keys_shift);
   return n > 0 ? n : 1;
 }
 
-// Steps of one kv head of a sequence.
-TSFA_HD inline int64_t head_steps(const Cut& c, const Seq& s) {
-  const int n = cut_tiles(c, s);
-  if (n == 0) return 0;
-  if (!c.causal) return (int64_t)n * tile_steps(c, s, 0);
-  int64_t sum = 0;
-  for (int r = 0; r < n; ++r) sum += tile_steps(c, s, r);
-  return sum;
+// Line lengths: tile 0 of a sequence and what each further tile adds to it,
+// the first r tiles, and one kv head.
+TSFA_HD inline int64_t tile_first(const Cut& c, const Seq& s) {
+  if (c.causal) return ((int64_t)s.prefix + 1) * c.group + c.rows - 1 + c.unit - 1;
+  return tile_steps(c, s, 0) * c.unit;
 }
+TSFA_HD inline int64_t tile_more(const Cut& c) { return c.causal ? c.rows : 0; }
+TSFA_HD inline int64_t tiles_length(const Cut& c, const Seq& s, int64_t r) {
+  return r * tile_first(c, s) + tile_more(c) * (r * (r - 1) / 2);
+}
+TSFA_HD inline int64_t head_length(const Cut& c, const Seq& s) { return tiles_length(c, s, cut_tiles(c, s)); }
 
-// A place on the line: the next step of `tile` of kv head `kvh` of sequence b.
+// A place on the line: a step of `tile` of kv head `kvh`; from: the line from
+// the tile's start to the given point.
 struct Place {
-  int b, kvh, tile, step;
-  Seq seq;
+  int kvh, tile, step;
+  int64_t from;
 };
 
-// The place `at` steps into sequence b (at < head_steps * num_kv_heads).
-TSFA_HD inline Place place_in_seq(const Cut& c, const Seq& s, int b, int64_t at) {
+// The first step at or behind the point x of a sequence's line (x < its
+// length); tile or kvh may come out one past the sequence's last.
+TSFA_HD inline Place place_in_seq(const Cut& c, const Seq& s, int64_t x) {
   Place p;
-  p.b = b;
-  p.seq = s;
-  const int64_t per = head_steps(c, s);
-  p.kvh = (int)(at / per);
-  int64_t left = at - p.kvh * per;
+  const int n = cut_tiles(c, s);
+  const int64_t head = head_length(c, s);
+  p.kvh = (int)udiv(x, head, 1.0 / (double)head);
+  x -= p.kvh * head;
+  const int64_t a = tile_first(c, s);
   if (!c.causal) {
-    const int n = tile_steps(c, s, 0);
-    p.tile = (int)(left / n);
-    p.step = (int)(left - (int64_t)p.tile * n);
-    return p;
+    p.tile = (int)udiv(x, a, 1.0 / (double)a);
+  } else {
+    // the last r with r a + rows r (r - 1) / 2 <= x
+    const double h = (double)a - 0.5 * c.rows;
+    int64_t r = (int64_t)((__builtin_sqrt(h * h + 2.0 * c.rows * (double)x) - h) / c.rows);
+    r = clamp64(r, 0, n - 1);
+    while (r > 0 && tiles_length(c, s, r) > x) --r;
+    while (r + 1 < n && tiles_length(c, s, r + 1) <= x) ++r;
+    p.tile = (int)r;
   }
-  p.tile = 0;
-  for (int n = tile_steps(c, s, 0); left >= n; n = tile_steps(c, s, ++p.tile)) left -= n;
-  p.step = (int)left;
+  p.from = x - tiles_length(c, s, p.tile);
+  p.step = (int)udiv(p.from + c.unit - 1, c.unit, c.inv_unit);
+  if (p.step >= tile_steps(c, s, p.tile)) {  // between the tile's last step and its end
+    p.from -= a + tile_more(c) * p.tile;
+    p.step = 0;
+    if (++p.tile == n) {
+      p.tile = 0;
+      ++p.kvh;
+    }
+  }
   return p;
+}
+
+// Length of a run, at least half a step's: with fewer steps than workgroups a
+// run holds one step or none.
+TSFA_HD inline int64_t run_length(const Cut& c, int64_t total, int groups) {
+  const int64_t per = udiv(total + groups - 1, groups, 1.0 / (double)groups);
+  return per > (c.unit + 1) / 2 ? per : (c.unit + 1) / 2;
+}
+// Steps of a tile that start before the line's point `ahead` past its start.
+TSFA_HD inline int steps_before(const Cut& c, int64_t ahead, int steps) {
+  if (ahead <= 0) return 0;
+  const int64_t n = udiv(ahead + c.unit - 1, c.unit, c.inv_unit);
+  return n < steps ? (int)n : steps;
+}
+// Whether the run at `at` holds steps of the tile at `tile` (each a point of
+// the line; the tile's steps come from udiv, exact below 2^52).
+TSFA_HD inline bool run_has_step(const Cut& c, int64_t at, int64_t per, int64_t tile) {
+  return per >= c.unit || steps_before(c, at + per - tile, INT32_MAX) > steps_before(c, at - tile, INT32_MAX);
 }
 
 // The part [from, end) of a tile's steps that runs in one go: its page ids

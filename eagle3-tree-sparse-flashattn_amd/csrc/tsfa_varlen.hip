@@ -57,7 +57,14 @@ struct Args {
   int num_heads, groups;           // workgroups on the line
   float4* ws_o;                    // [2 * groups][RG][D / 8][64] unnormalised O, a lane's registers in order
   float2* ws_ml;                   // [2 * groups][rows] (m, l)
-  int4* ws_desc;                   // [groups] the tile that starts in the run and ends behind it
+  // [groups] the tile that starts in the run and ends behind it: sequence, kv
+  // head, tile and how many runs on it ends (0: none), its place on the line,
+  // a run's length
+  struct Desc {
+    int b, kvh, tile, runs;
+    int64_t at, per;
+  };
+  Desc* ws_desc;
 };
 
 // Layout of 32-key tiles of D elements: key row k, 16-byte chunk c at chunk
@@ -83,6 +90,28 @@ __device__ inline void dma_1k(const void* base, uint32_t off, uint32_t lds_in) {
                : "v"(off), "s"(sbase), "s"(lds)
                : "memory", "m0");
 }
+// N such loads to consecutive LDS KBs from one base: load i reads base +
+// off[i] + i KB (the immediate offset counts for both addresses).
+template <int N> __device__ inline void dma_rows(const void* base, const uint32_t (&off)[N], uint32_t lds_in) {
+  static_assert(N == 2 || N == 4, "16 key rows");
+  const uint64_t u = reinterpret_cast<uint64_t>(base);
+  const uint64_t sbase = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(u >> 32)) << 32) |
+                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)u);
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_in);
+  if constexpr (N == 4)
+    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
+                 :
+                 : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(sbase), "s"(lds)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                 :
+                 : "v"(off[0]), "v"(off[1]), "s"(sbase), "s"(lds)
+                 : "memory", "m0");
+}
 #pragma clang diagnostic pop
 template <int N> __device__ inline void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 // At most `left` units of LPW loads each still on their way (left <= K).
@@ -96,59 +125,55 @@ template <int LPW, int K> __device__ inline void wait_units(int left) {
 }
 __device__ inline void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The place of the line's step `at`, and the line's length in *total; every
-// lane of a wave calls it and gets the same answer.  Lanes take 64 sequences
-// at a time.
-__device__ inline int64_t lane_scan(int64_t x, int lane) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int64_t y = __shfl_up(x, s);
-    if (lane >= s) x += y;
-  }
-  return x;
-}
 __device__ inline int64_t uniform64(int64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
-struct Line {
-  int64_t total, per;  // steps in all, steps of one workgroup
-  int used;            // workgroups with work
+__device__ inline int64_t readlane64(int64_t x, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, l);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), l);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// x of the lane that the DPP control names, 0 where there is none.
+template <int CTRL, int ROWS> __device__ inline int64_t dpp64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)((uint64_t)x >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// Sums over the lanes up to each one, without LDS: shifts within rows of 16,
+// then the last lane of row 0 (2) to row 1 (3), of row 1 to rows 2 and 3.
+__device__ inline int64_t lane_scan(int64_t x) {
+  x += dpp64<0x111, 0xf>(x);
+  x += dpp64<0x112, 0xf>(x);
+  x += dpp64<0x114, 0xf>(x);
+  x += dpp64<0x118, 0xf>(x);
+  x += dpp64<0x142, 0xa>(x);
+  x += dpp64<0x143, 0xc>(x);
+  return x;
+}
+
+// The sequences in a wave's registers, lane l holding sequence b0 + l.
+struct LaneSeqs {
+  int b0;
+  Seq mine;
+  __device__ void load(const paged::Seqs& s, int from, int lane) {
+    b0 = from;
+    mine = Seq{};
+    if (b0 + lane < s.batch) mine = paged::seq_of(s, b0 + lane);
+  }
+  __device__ int64_t length(const Cut& c) const { return paged::head_length(c, mine) * c.num_kv_heads; }
+  __device__ Seq at(int l) const {
+    Seq r;
+    r.q0 = __builtin_amdgcn_readlane(mine.q0, l);
+    r.q_len = __builtin_amdgcn_readlane(mine.q_len, l);
+    r.kv_len = __builtin_amdgcn_readlane(mine.kv_len, l);
+    r.prefix = __builtin_amdgcn_readlane(mine.prefix, l);
+    r.list = readlane64(mine.list, l);
+    r.pages = __builtin_amdgcn_readlane(mine.pages, l);
+    return r;
+  }
 };
-__device__ inline Line line_of(const paged::Seqs& s, const Cut& c, int groups, int lane) {
-  int64_t sum = 0;
-  for (int b0 = 0; b0 < s.batch; b0 += 64) {
-    const int b = b0 + lane;
-    int64_t x = b < s.batch ? paged::head_steps(c, paged::seq_of(s, b)) * c.num_kv_heads : 0;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-    sum += uniform64(x);
-  }
-  Line l;
-  l.total = sum;
-  l.per = (sum + groups - 1) / groups;
-  l.used = sum > 0 ? (int)((sum + l.per - 1) / l.per) : 0;
-  return l;
-}
-__device__ inline Place place_at(const paged::Seqs& s, const Cut& c, int64_t at, int lane) {
-  for (int b0 = 0; b0 < s.batch; b0 += 64) {
-    const int b = b0 + lane;
-    const int64_t mine = b < s.batch ? paged::head_steps(c, paged::seq_of(s, b)) * c.num_kv_heads : 0;
-    const int64_t upto = lane_scan(mine, lane);
-    const uint64_t past = __ballot(upto > at);
-    if (past != 0) {
-      const int l = __builtin_ctzll(past);
-      const int64_t before = uniform64(__shfl(upto - mine, l));
-      const int bb = __builtin_amdgcn_readfirstlane(b0 + l);
-      return paged::place_in_seq(c, paged::seq_of(s, bb), bb, at - before);
-    }
-    at -= uniform64(__shfl(upto, 63));
-  }
-  Place none;
-  none.b = -1;  // not reached with at < total
-  return none;
-}
 
 // The logical run of a workgroup: neighbouring runs share K/V units, so the
 // runs are dealt to the 8 XCDs (block id modulo 8) in contiguous eighths.
@@ -181,7 +206,10 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   // two elements' exponent bits, and what carries all-ones exponents into bit 15
   constexpr uint32_t EXP2 = std::is_same<T, __bf16>::value ? 0x7f807f80u : 0x7c007c00u;
   constexpr uint32_t ONE2 = std::is_same<T, __bf16>::value ? 0x00800080u : 0x04000400u;
-  static_assert(LPW >= 1 && LPW * (NST - 1) < 64 && NST >= 2, "ring");
+  constexpr int GL = 16 / RPL;    // loads of 16 key rows (never more than a page)
+  constexpr int NG = LPW / GL;    // groups of 16 rows a wave moves per unit
+  constexpr bool PIPE = NST >= 4;  // the next unit's scores run under this unit's softmax
+  static_assert(NG >= 1 && LPW % GL == 0 && LPW * (NST - 1) < 64 && NST >= 2, "ring");
   extern __shared__ __attribute__((aligned(256))) unsigned char smem[];
   int32_t* table = reinterpret_cast<int32_t*>(smem + C::kRing);
   uint32_t* words = reinterpret_cast<uint32_t*>(smem + C::kRing + kTableIds * 4);
@@ -194,28 +222,81 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   const int G = cut.group;
 
   const int run = run_of_block(blockIdx.x, a.groups);
-  const Line line = line_of(a.seqs, cut, a.groups, lane);
-  if (tid == 0) a.ws_desc[run] = make_int4(0, 0, 0, 0);
-  if (run >= line.used) return;
-  int64_t at = run * line.per;
-  const int64_t end = at + line.per < line.total ? at + line.per : line.total;
-  Place pl = place_at(a.seqs, cut, at, lane);
-  if (pl.b < 0) return;
+  if (tid == 0) a.ws_desc[run].runs = 0;
+  LaneSeqs seqs;
+  seqs.load(a.seqs, 0, lane);
+  int64_t upto = lane_scan(seqs.length(cut));  // of chunk 0
+  int64_t total = readlane64(upto, 63);
+  if (a.seqs.batch > 64) {
+    for (int b0 = 64; b0 < a.seqs.batch; b0 += 64) {
+      seqs.load(a.seqs, b0, lane);
+      total += readlane64(lane_scan(seqs.length(cut)), 63);
+    }
+    seqs.load(a.seqs, 0, lane);
+  }
+  const int64_t per = uniform64(paged::run_length(cut, total, a.groups));
+  int64_t at = run * per;  // the run: [at, end) of the line
+  if (at >= total) return;
+  const int64_t end = at + per < total ? at + per : total;
+  int64_t before = 0;  // the line before chunk b0
+  while (before + readlane64(upto, 63) <= at) {
+    before += readlane64(upto, 63);
+    if (seqs.b0 + 64 >= a.seqs.batch) return;  // not reached: at < total
+    seqs.load(a.seqs, seqs.b0 + 64, lane);
+    upto = lane_scan(seqs.length(cut));
+  }
+  int sl = __builtin_ctzll(__ballot(before + upto > at));
+  Seq sq = seqs.at(sl);
+  Place pl;
+  {
+    const int64_t start = before + readlane64(upto, sl) - uniform64(paged::head_length(cut, sq)) * cut.num_kv_heads;
+    const Place p = paged::place_in_seq(cut, sq, at - start);
+    pl.kvh = __builtin_amdgcn_readfirstlane(p.kvh);
+    pl.tile = __builtin_amdgcn_readfirstlane(p.tile);
+    pl.step = __builtin_amdgcn_readfirstlane(p.step);
+    pl.from = uniform64(p.from);
+  }
+  int64_t left = end - (at - pl.from);  // from the tile's start to the run's end
+  // the next sequence with query rows; false behind the last
+  auto next_seq = [&]() {
+    do {
+      if (seqs.b0 + ++sl >= a.seqs.batch) return false;
+      if (sl == 64) {
+        seqs.load(a.seqs, seqs.b0 + 64, lane);
+        sl = 0;
+      }
+      sq = seqs.at(sl);
+    } while (sq.q_len == 0);
+    return true;
+  };
+  if (pl.kvh == cut.num_kv_heads) {
+    pl.kvh = 0;
+    if (!next_seq()) return;
+  }
 
-  // the wave's share of a unit: rows [row0, row0 + rows) of K or V
-  constexpr int HALF = LPW * RG / 2;  // loads of one tile
+  // The wave's share of a unit: groups rg NG .. rg NG + NG - 1 of 16 key rows
+  // (groups 0 and 1 are K's, 2 and 3 V's).  Chunk x of row k lies at chunk x ^
+  // swz(k), and both swizzles have a period that divides 16.
   const uint32_t ring = lds_addr(smem) + (uint32_t)(st * NST * C::kUnit);
+  uint32_t off_k[GL], off_v[GL];
+#pragma unroll
+  for (int i = 0; i < GL; ++i) {
+    const int row = i * RPL + lane / CPR;
+    const uint32_t at_row = (uint32_t)row * (uint32_t)a.cr * 2u - (uint32_t)i * 1024u;
+    off_k[i] = at_row + (uint32_t)(((lane % CPR) ^ swz_k<D>(row)) << 4);
+    off_v[i] = at_row + (uint32_t)(((lane % CPR) ^ swz_v<D>(row)) << 4);
+  }
 
   for (;;) {
-    const int b = pl.b;
-    const Seq sq = pl.seq;
+    const int b = seqs.b0 + sl;
     const int n_steps = paged::tile_steps(cut, sq, pl.tile);
     const int s0 = pl.step;
-    const int s1 = (int)(end - at < n_steps - s0 ? s0 + (end - at) : n_steps);
+    const int s1 = __builtin_amdgcn_readfirstlane(paged::steps_before(cut, left, n_steps));
+    if (s0 >= s1) return;
     const int TG = sq.q_len * G;
     const int r = pl.tile * M + rg * 32 + ln;
     const int R = min(r, TG - 1);
-    const int t = R / G, g = R - t * G;
+    const int t = (int)fdiv((uint32_t)R, cut.by_group), g = R - t * G;
     const float sl2 = a.scale_log2;
 
     // Q^T operand: lane (ln, lh) holds d = 16 kk + 8 lh + [0, 8) of its row
@@ -238,6 +319,9 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     const T* hbase = static_cast<const T*>(a.cache) + pl.kvh * a.ch;
     const int kl = sq.kv_len, P = sq.prefix;
     const int mask_cols = a.mask != nullptr ? min(min(sq.q_len, a.mask_n), kl - P) : 0;
+    // keys that every row of the tile sees: the prefix, or up to the tile's
+    // first token's own
+    const int seen_by_all = a.mask != nullptr ? P : min(kl, P + (int)fdiv((uint32_t)(pl.tile * M), cut.by_group) + 1);
     const uint8_t* mask_seq = a.mask != nullptr ? a.mask + b * a.mask_seq : nullptr;
 
     // visibility of keys k0 .. k0 + 31 for token t
@@ -265,83 +349,127 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       if (a.mask != nullptr) {
         for (int i = tid; i < (c1 * S - ut0) * M; i += C::kWaves * 64) {
           const int row = min(pl.tile * M + i % M, TG - 1);
-          words[i] = word_of((ut0 + i / M) * 32, row / G);
+          words[i] = word_of((ut0 + i / M) * 32, (int)fdiv((uint32_t)row, cut.by_group));
         }
       }
       barrier();
 
-      // Unit j of the chunk's stream into stage j % NST.  Load i of the wave
-      // moves RPL key rows (never more than a page); rows past the last key
-      // repeat a valid one, so that no stale value of the pool enters P V.
+      // Unit j of the chunk's stream into stage j % NST.  Units that reach past
+      // the last key take their rows load by load, each from a block that holds
+      // a key, so that no stale value of the pool enters P V.
       const int n = c1 - c0;
       auto issue = [&](int j) {
         const int k0 = ((c0 + j) * S + st) * 32;
         const uint32_t dst = ring + (uint32_t)((j % NST) * C::kUnit);
+        if (k0 + 32 <= kl) {
 #pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-          const int u = rg * LPW + i;          // load of the unit: K's, then V's
-          const bool is_v = u >= HALF;
-          const int kb = (is_v ? u - HALF : u) * RPL;
-          const int blk = paged::load_block(k0 + kb, RPL, kl);
-          const int id = __builtin_amdgcn_readfirstlane(table[min((blk >> ps) - first_page, kTableIds - 1)]);
-          const T* base = hbase + id * a.cp + (is_v ? a.cs : 0) + (int64_t)(blk & ((1 << ps) - 1)) * a.cr;
-          const int row = kb + lane / CPR;
-          const int from = min(lane / CPR, kl - 1 - blk);
-          const int chunk = (lane % CPR) ^ (is_v ? swz_v<D>(row) : swz_k<D>(row));
-          dma_1k(base, (uint32_t)from * (uint32_t)a.cr * 2u + (uint32_t)chunk * 16u, dst + (uint32_t)u * 1024u);
+          for (int x = 0; x < NG; ++x) {
+            const int grp = rg * NG + x;
+            const int key = k0 + 16 * (grp & 1);
+            const int id = __builtin_amdgcn_readfirstlane(table[(key >> ps) - first_page]);
+            const T* base = hbase + id * a.cp + (grp >= 2 ? a.cs : 0) + (int64_t)(key & ((1 << ps) - 1)) * a.cr;
+            if (grp >= 2) dma_rows<GL>(base, off_v, dst + (uint32_t)grp * (GL * 1024u));
+            else dma_rows<GL>(base, off_k, dst + (uint32_t)grp * (GL * 1024u));
+          }
+        } else {
+          for (int x = 0; x < LPW; ++x) {
+            const int u = rg * LPW + x;  // load of the unit
+            const bool is_v = u >= 2 * GL;
+            const int kb = (u % (2 * GL)) * RPL;
+            const int blk = paged::load_block(k0 + kb, RPL, kl);
+            const int id = __builtin_amdgcn_readfirstlane(table[(blk >> ps) - first_page]);
+            const T* base = hbase + id * a.cp + (is_v ? a.cs : 0) + (int64_t)(blk & ((1 << ps) - 1)) * a.cr;
+            const int row = kb + lane / CPR;
+            const int from = min(lane / CPR, kl - 1 - blk);
+            const int chunk = (lane % CPR) ^ (is_v ? swz_v<D>(row) : swz_k<D>(row));
+            dma_1k(base, (uint32_t)from * (uint32_t)a.cr * 2u + (uint32_t)chunk * 16u, dst + (uint32_t)u * 1024u);
+          }
         }
       };
 
-      vm_wait<0>();  // the ring's waits count its own loads alone
-      for (int j = 0; j < NST - 1 && j < n; ++j) issue(j);
-      for (int j = 0; j < n; ++j) {
-        wait_units<LPW, NST - 2>(min(n - 1 - j, NST - 2));
-        barrier();  // unit j is there, and every wave is done with unit j - 1
-        if (j + NST - 1 < n) issue(j + NST - 1);
-
-        const unsigned char* kt = smem + (st * NST + j % NST) * C::kUnit;
-        const unsigned char* vt = kt + C::kTile;
-        const int u = (c0 + j) * S + st;
-
-        // S^T: lane (ln, lh) element i is key 8 (i / 4) + 4 lh + i % 4 of row ln
+      // S^T of the unit at kt: lane (ln, lh) element i is key 8 (i / 4) + 4 lh
+      // + i % 4 of row ln.  K is read KA steps ahead, fenced (left alone, the
+      // compiler reads one step ahead and each MFMA waits an LDS latency);
+      // between() runs after the first reads, slice(kk) after MFMA kk.
+      auto scores = [&](const unsigned char* kt, auto between, auto slice) {
+        constexpr int KA = 4;
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        i16x8 kf[KS];
+        auto rk = [&](int kk) {
+          kf[kk] = *reinterpret_cast<const i16x8*>(kt + ln * C::kRowBytes + (((2 * kk + lh) ^ swz_k<D>(ln)) << 4));
+        };
+#pragma unroll
+        for (int kk = 0; kk < KA; ++kk) rk(kk);
+        __builtin_amdgcn_sched_barrier(0);
+        between();
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
-          const i16x8 kf = *reinterpret_cast<const i16x8*>(kt + ln * C::kRowBytes + (((2 * kk + lh) ^ swz_k<D>(ln)) << 4));
-          s = Mma<T>::run(bit_cast<V8>(kf), bit_cast<V8>(qf[kk]), s);
+          if (kk + KA < KS) rk(kk + KA);
+          s = Mma<T>::run(bit_cast<V8>(kf[kk]), bit_cast<V8>(qf[kk]), s);
+          slice(kk);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        const bool masked = (u + 1) * 32 > P;
+        return s;
+      };
+      auto none = [](auto...) {};
+
+      // Unit j, whose scores are in s: online softmax, O^T += V^T P^T.  NEXT: a
+      // unit that every row sees whole, unit j + 1's scores (left in s) between
+      // its exponentials; else the unit may need its mask and stands alone.
+      auto unit = [&](auto next_c, int j, f32x16& s) {
+        constexpr bool NEXT = decltype(next_c)::value;
+        const unsigned char* vt = smem + (st * NST + j % NST) * C::kUnit + C::kTile;
+        const int u = (c0 + j) * S + st;
+        const bool masked = !NEXT && (u + 1) * 32 > seen_by_all;
         uint32_t w = 0xffffffffu;
-        if (masked) {
-          w = a.mask != nullptr ? words[(u - ut0) * M + rg * 32 + ln] : word_of(u * 32, t);
+        float alpha, ms;
+        bool need;
+        auto stats = [&]() {
+          if (masked) {
+            w = a.mask != nullptr ? words[(u - ut0) * M + rg * 32 + ln] : word_of(u * 32, t);
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!((w >> (8 * (i >> 2) + 4 * lh + (i & 3))) & 1u)) s[i] = -INFINITY;
-        }
-        float mx = s[0];
+            for (int i = 0; i < 16; ++i)
+              if (!((w >> (8 * (i >> 2) + 4 * lh + (i & 3))) & 1u)) s[i] = -INFINITY;
+          }
+          float mx = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        const float rmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        // the reference point moves only when a score passes it by more than
-        // 2^8 (exact for any consistent point; p stays below 2^8)
-        const bool need = rmax > m_lim;
-        const float m_new = need ? rmax : m_run;
-        const float alpha = need ? __builtin_amdgcn_exp2f((m_run - m_new) * sl2) : 1.f;
-        m_run = m_new;
-        m_lim = m_new + thr;
-        const float ms = m_new == -INFINITY ? 0.f : m_new;
-        // P is rounded to the input type for the product with V; its row sum
-        // takes the unrounded values
-        float psum = 0.f;
+          for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          const float rmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          // the reference point moves only when a score passes it by more than
+          // 2^8 (exact for any consistent point; p stays below 2^8)
+          need = rmax > m_lim;
+          const float m_new = need ? rmax : m_run;
+          alpha = need ? __builtin_amdgcn_exp2f((m_run - m_new) * sl2) : 1.f;
+          m_run = m_new;
+          m_lim = m_new + thr;
+          ms = m_new == -INFINITY ? 0.f : m_new;
+        };
+        // P is rounded to the input type for the product with V, which takes
+        // 16-bit operands; its row sum takes the unrounded values.  Pinned where
+        // they are computed: the compiler sinks them past the re-base otherwise.
+        float psum = 0.f, p[16];
         uint32_t pk[8];
+        auto expo = [&](int i) {
+          p[i] = __builtin_amdgcn_exp2f((s[i] - ms) * sl2);
+          psum += p[i];
+          if (i & 1) {
+            pk[i >> 1] = bit_cast<uint32_t>(T2{(T)p[i - 1], (T)p[i]});
+            asm volatile("" : "+v"(pk[i >> 1]), "+v"(psum));
+          }
+        };
+        if constexpr (NEXT) {
+          const f32x16 sn = scores(smem + (st * NST + (j + 1) % NST) * C::kUnit, stats, [&](int kk) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float p0 = __builtin_amdgcn_exp2f((s[i] - ms) * sl2), p1 = __builtin_amdgcn_exp2f((s[i + 1] - ms) * sl2);
-          psum += p0 + p1;
-          pk[i >> 1] = bit_cast<uint32_t>(T2{(T)p0, (T)p1});
+            for (int i = 16 / KS * kk; i < 16 / KS * (kk + 1); ++i) expo(i);
+          });
+          s = sn;
+        } else {
+          stats();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) expo(i);
         }
         l_run = l_run * alpha + psum;
         if (__ballot(need) != 0) {
@@ -349,14 +477,23 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
         }
 
-        // O^T += V^T P^T; V^T by the transposing LDS read: lane i of 16-lane
-        // group x gets keys 16 s2 + 8 jj + 4 (x >> 1) + [0, 4) of
-        // d = 32 dt + 16 (x & 1) + i, the key order in which P lies
+        // V^T by the transposing LDS read: lane i of 16-lane group x gets keys
+        // 16 s2 + 8 jj + 4 (x >> 1) + [0, 4) of d = 32 dt + 16 (x & 1) + i, the
+        // key order in which P lies
         const V8 pb[2] = {bit_cast<V8>(U4{pk[0], pk[1], pk[2], pk[3]}), bit_cast<V8>(U4{pk[4], pk[5], pk[6], pk[7]})};
         const int vx = lane >> 4, vi = lane & 15;
         const int vrow = 4 * (vx >> 1) + (vi >> 2);
         const int vch = 2 * (vx & 1) + ((vi & 3) >> 1), vhalf = 8 * (vi & 1);
         const uint32_t vb = lds_addr(vt) + (uint32_t)(vrow * C::kRowBytes + vhalf);
+        i16x4 vh[2 * DT][2];
+        auto rv = [&](int x) {
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj)
+            vh[x][jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (TSFA_LDS i16x4*)(uintptr_t)(vb + (uint32_t)((16 * (x & 1) + 8 * jj) * C::kRowBytes +
+                                                             (((4 * (x >> 1) + vch) ^ swz_v<D>(vrow)) << 4))));
+        };
+        auto vf = [&](int x) { return __builtin_shufflevector(vh[x][0], vh[x][1], 0, 1, 2, 3, 4, 5, 6, 7); };
         bool odd = false;
         if (masked) {
           // infinities and NaN of keys that some rows do not see: 0 * NaN must
@@ -371,191 +508,283 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           }
           odd = __ballot(hit != 0) != 0;
         }
+        constexpr int VA = 3;
+#pragma unroll
+        for (int x = 0; x < VA; ++x) rv(x);
 #pragma unroll
         for (int x = 0; x < 2 * DT; ++x) {
-          const int dt = x >> 1, s2 = x & 1;
-          i16x4 h[2];
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int row = 16 * s2 + 8 * jj;  // swz_v has period 8 in the key
-            h[jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (TSFA_LDS i16x4*)(uintptr_t)(vb + (uint32_t)(row * C::kRowBytes + (((4 * dt + vch) ^ swz_v<D>(vrow)) << 4))));
-          }
-          i16x8 vf = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-          if (odd) {
+          if (x + VA < 2 * DT) rv(x + VA);
+          i16x8 f = vf(x);
+          if (!NEXT && odd) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if ((vf[e] & (short)(EXP2 & 0xffff)) == (short)(EXP2 & 0xffff)) vf[e] = 0;
+              if ((f[e] & (short)(EXP2 & 0xffff)) == (short)(EXP2 & 0xffff)) f[e] = 0;
           }
-          o[dt] = Mma<T>::run(bit_cast<V8>(vf), pb[s2], o[dt]);
+          o[x >> 1] = Mma<T>::run(bit_cast<V8>(f), pb[x & 1], o[x >> 1]);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if (odd) {
+        if (!NEXT && odd) {
+#pragma unroll 1
           for (int key = 0; key < 32; ++key) {
-            if (!((w >> key) & 1u)) continue;
+            const bool seen = (w >> key) & 1u;
+            const unsigned char* row = vt + key * C::kRowBytes + 8 * lh;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+            for (int x = 0; x < D / 8; ++x) {
+              const T4 v = *reinterpret_cast<const T4*>(row + ((x ^ swz_v<D>(key)) << 4));
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int d = 32 * dt + 8 * (i >> 2) + 4 * lh + (i & 3);
-                const float v = (float)*reinterpret_cast<const T*>(vt + key * C::kRowBytes +
-                                                                   (((d >> 3) ^ swz_v<D>(key)) << 4) + 2 * (d & 7));
-                if (!(v - v == 0.f)) o[dt][i] += v;
+              for (int e = 0; e < 4; ++e) {
+                const float f = (float)v[e];
+                o[x >> 2][4 * (x & 3) + e] += seen && !(f - f == 0.f) ? f : 0.f;
               }
+            }
           }
         }
+      };
+
+      vm_wait<0>();  // the ring's waits count its own loads alone
+      for (int j = 0; j < NST - 1 && j < n; ++j) issue(j);
+      int issued = min(n, NST - 1), j = 0;
+      wait_units<LPW, NST - 2>(issued - 1);
+      barrier();
+      f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
+      if constexpr (PIPE) {
+        // steps whose units every row of the tile sees whole
+        const int n_full = min(n, seen_by_all / (32 * S) - c0);
+        for (; j + 1 < n_full; ++j) {
+          // unit j + 1 is there, and every wave is done with unit j - 1
+          wait_units<LPW, NST - 3>(issued - 2 - j);
+          barrier();
+          if (issued < n) issue(issued++);
+          unit(std::true_type{}, j, s);
+        }
+      }
+      for (;;) {
+        unit(std::false_type{}, j, s);
+        if (++j >= n) break;
+        wait_units<LPW, NST - 2>(issued - 1 - j);
+        barrier();  // unit j is there, and every wave is done with unit j - 1
+        while (issued < min(n, j + NST)) issue(issued++);
+        s = scores(smem + (st * NST + j % NST) * C::kUnit, none, none);
       }
       barrier();  // the rings, the table and the words are free again
       c0 = c1;
     }
     l_run += __shfl_xor(l_run, 32);
 
-    // The streams' results join in LDS: streams 1 .. S - 1 leave (m, l, O) in
-    // the ring, stream 0 takes them in.
-    if constexpr (S > 1) {
-      float4* jo = reinterpret_cast<float4*>(smem);                                  // [S - 1][RG][D / 8][64]
-      float2* jml = reinterpret_cast<float2*>(smem + (S - 1) * RG * (D / 8) * 1024);  // [S - 1][RG][32]
-      static_assert((S - 1) * RG * (D / 8) * 1024 + (S - 1) * RG * 32 * 8 <= C::kRing, "join");
-      if (st > 0) {
-        const int x = (st - 1) * RG + rg;
+    // The streams' results join in LDS, every wave finishing 1 / S of its row
+    // group's columns: a lane's float4 x holds d = 8 x + 4 lh .. + 3, stream s
+    // takes x in [s X / S, (s + 1) X / S).
+    constexpr int X = D / 8, XS = X / S;
+    const bool whole = s0 == 0 && s1 == n_steps;
+    float4* jo = reinterpret_cast<float4*>(smem);                              // the streams' O
+    float2* jml = reinterpret_cast<float2*>(smem + C::kRing + kTableIds * 4);  // [S][RG][32] (m, l)
+    static_assert(S * RG * 32 * 8 <= C::kWords && S * RG * X * 1024 <= C::kRing, "join");
+    if (lh == 0) jml[(st * RG + rg) * 32 + ln] = make_float2(m_run, l_run);
+    float mm = -INFINITY, ll = 0.f, fs[S];
+    auto weights = [&]() {
+      float2 ml[S];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            jo[(x * (D / 8) + 4 * dt + i) * 64 + lane] =
-                make_float4(o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]);
-        if (lh == 0) jml[x * 32 + ln] = make_float2(m_run, l_run);
+      for (int i = 0; i < S; ++i) {
+        ml[i] = jml[(i * RG + rg) * 32 + ln];
+        mm = fmaxf(mm, ml[i].x);
       }
-      barrier();
-      if (st == 0) {
+      const float m0 = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-        for (int s = 1; s < S; ++s) {
-          const int x = (s - 1) * RG + rg;
-          const float2 ml = jml[x * 32 + ln];
-          const float m_new = fmaxf(m_run, ml.x);
-          const float m0 = m_new == -INFINITY ? 0.f : m_new;
-          const float fa = __builtin_amdgcn_exp2f((m_run - m0) * sl2), fb = __builtin_amdgcn_exp2f((ml.x - m0) * sl2);
-          m_run = m_new;
-          l_run = l_run * fa + ml.y * fb;
+      for (int i = 0; i < S; ++i) {
+        fs[i] = __builtin_amdgcn_exp2f((ml[i].x - m0) * sl2);
+        ll += ml[i].y * fs[i];
+      }
+    };
+    // a tile of one run: O; a shared one: slot 2 run if it began before the
+    // run, else 2 run + 1
+    T* orow = static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)(pl.kvh * G + g) * a.soh + 4 * lh;
+    const int64_t slot = 2 * (int64_t)run + (s0 == 0 ? 1 : 0);
+    float4* wo = a.ws_o + (slot * RG + rg) * X * 64 + lane;
+    auto put = [&](int x, float4 v) {
+      if (whole) {
+        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);  // NaN stays
+        const T4 r4 = {(T)(v.x * inv), (T)(v.y * inv), (T)(v.z * inv), (T)(v.w * inv)};
+        if (r < TG) *reinterpret_cast<T4*>(orow + 8 * x) = r4;
+      } else {
+        wo[x * 64] = v;
+      }
+    };
+    auto o4 = [&](int x) {
+      const int dt = x >> 2, i = x & 3;
+      return make_float4(o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]);
+    };
+    if constexpr (S == 2) {
+      // each stream leaves the other's half and finishes its own
+      float4* mine = jo + ((st * RG + rg) * XS) * 64 + lane;
+      const float4* other = jo + (((1 - st) * RG + rg) * XS) * 64 + lane;
+      auto half = [&](auto st_c) {
+        constexpr int ST = decltype(st_c)::value;
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
+        for (int x = 0; x < XS; ++x) mine[x * 64] = o4((1 - ST) * XS + x);
+        barrier();
+        weights();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float4 v = jo[(x * (D / 8) + 4 * dt + i) * 64 + lane];
-              o[dt][4 * i] = o[dt][4 * i] * fa + v.x * fb;
-              o[dt][4 * i + 1] = o[dt][4 * i + 1] * fa + v.y * fb;
-              o[dt][4 * i + 2] = o[dt][4 * i + 2] * fa + v.z * fb;
-              o[dt][4 * i + 3] = o[dt][4 * i + 3] * fa + v.w * fb;
-            }
+        for (int x = 0; x < XS; ++x) {
+          const float4 u = o4(ST * XS + x), v = other[x * 64];
+          put(ST * XS + x, make_float4(u.x * fs[ST] + v.x * fs[1 - ST], u.y * fs[ST] + v.y * fs[1 - ST],
+                                       u.z * fs[ST] + v.z * fs[1 - ST], u.w * fs[ST] + v.w * fs[1 - ST]));
         }
+      };
+      if (st == 0) half(std::integral_constant<int, 0>{});
+      else half(std::integral_constant<int, 1>{});
+    } else {
+#pragma unroll
+      for (int x = 0; x < X; ++x) jo[((st * RG + rg) * X + x) * 64 + lane] = o4(x);
+      barrier();
+      weights();
+#pragma unroll
+      for (int y = 0; y < XS; ++y) {
+        const int x = st * XS + y;
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const float4 v = jo[((i * RG + rg) * X + x) * 64 + lane];
+          u.x += v.x * fs[i];
+          u.y += v.y * fs[i];
+          u.z += v.z * fs[i];
+          u.w += v.w * fs[i];
+        }
+        put(x, u);
       }
     }
-
-    if (st == 0) {
-      if (s0 == 0 && s1 == n_steps) {
-        if (r < TG) {
-          const float inv = l_run > 0.f ? 1.f / l_run : (l_run == 0.f ? 0.f : l_run);  // NaN stays
-          T* orow = static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)(pl.kvh * G + g) * a.soh;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              T4 v;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = (T)(o[dt][4 * i + e] * inv);
-              *reinterpret_cast<T4*>(orow + 32 * dt + 8 * i + 4 * lh) = v;
-            }
-          if (a.lse != nullptr && lh == 0)
-            a.lse[(int64_t)(sq.q0 + t) * a.num_heads + pl.kvh * G + g] =
-                l_run == 0.f ? -INFINITY : m_run * (sl2 * 0.6931471805599453f) + logf(l_run);
-        }
-      } else {
-        // shared tile: slot 2 run if it began before this run, else 2 run + 1
-        const int64_t slot = 2 * (int64_t)run + (s0 == 0 ? 1 : 0);
-        float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8)) * 64 + lane;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            wo[(4 * dt + i) * 64] = make_float4(o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]);
-        if (lh == 0) a.ws_ml[slot * M + rg * 32 + ln] = make_float2(m_run, l_run);
-        if (s0 == 0 && wave == 0 && lane == 0) {
-          const int64_t last = (at + n_steps - 1) / line.per;
-          a.ws_desc[run] = make_int4(b, pl.kvh, pl.tile, (int)(last - run) + 1);
-        }
+    if (st == 0 && lh == 0) {
+      if (!whole) {
+        a.ws_ml[slot * M + rg * 32 + ln] = make_float2(mm, ll);
+      } else if (a.lse != nullptr && r < TG) {
+        a.lse[(int64_t)(sq.q0 + t) * a.num_heads + pl.kvh * G + g] =
+            ll == 0.f ? -INFINITY : mm * (sl2 * 0.6931471805599453f) + logf(ll);
       }
+    }
+    if (tid == 0 && s0 == 0 && s1 < n_steps) {
+      const int64_t tile_at = end - left;  // the run that the tile's last step starts in:
+      const int64_t last = paged::udiv(tile_at + (n_steps - 1) * cut.unit, per, 1.0 / (double)per);
+      a.ws_desc[run] = Args::Desc{b, pl.kvh, pl.tile, (int)(last - run) + 1, tile_at, per};
     }
 
     // on along the line
-    at += s1 - s0;
-    if (at >= end) return;
-    if constexpr (S > 1) barrier();  // the ring is written again
+    if (s1 < n_steps) return;
+    barrier();  // the ring is written again
+    left -= paged::tile_first(cut, sq) + paged::tile_more(cut) * pl.tile;
+    if (left <= 0) return;
     pl.step = 0;
     if (++pl.tile == paged::cut_tiles(cut, sq)) {
       pl.tile = 0;
       if (++pl.kvh == cut.num_kv_heads) {
         pl.kvh = 0;
-        do {
-          if (++pl.b >= a.seqs.batch) return;  // not reached: steps are left, so some sequence has them
-          pl.seq = paged::seq_of(a.seqs, pl.b);
-        } while (paged::cut_tiles(cut, pl.seq) == 0);
+        if (!next_seq()) return;
       }
     }
   }
 }
 
 // Joins the parts of the tiles that several runs share: block (run, row
-// group); wave w takes d tiles w, w + 4, ...
+// group), a wave to every d tile and, with few row groups, PS waves that split
+// the parts; kJoin parts loaded at once.
+constexpr int kJoin = 4;
+template <int RG> constexpr int join_split() { return RG == 1 ? 4 : 1; }
 template <typename T, int D, int RG>
-__global__ __launch_bounds__(256) void combine_kernel(const Args a) {
+__global__ __launch_bounds__(join_split<RG>() * D * 2) void combine_kernel(const Args a) {
   typedef T T4 __attribute__((ext_vector_type(4)));
+  constexpr int DT = D / 32, PS = join_split<RG>(), M = 32 * RG;
+  __shared__ float4 jo[PS > 1 ? PS * DT * 4 * 64 : 1];
+  __shared__ float2 jml[PS > 1 ? PS * DT * 64 : 1];
   const int run = blockIdx.x, rg = blockIdx.y;
-  const int4 desc = a.ws_desc[run];
-  const int parts = desc.w;
+  const Args::Desc desc = a.ws_desc[run];
+  const int parts = desc.runs;
   if (parts == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int ln = lane & 31, lh = lane >> 5;
-  constexpr int M = 32 * RG;
-  const Seq sq = paged::seq_of(a.seqs, desc.x);
+  const int dt = wave % DT, ps = wave / DT;
+  const Seq sq = paged::seq_of(a.seqs, desc.b);
   const int G = a.cut.group, TG = sq.q_len * G;
-  const int r = desc.z * M + rg * 32 + ln;
-  if (r >= TG) return;
-  const int t = r / G, g = r - t * G;
-  auto slot_of = [&](int p) { return p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p); };
-  const float2* ml = a.ws_ml + rg * 32 + ln;
-  float m = -INFINITY;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[slot_of(p) * M].x);
-  const float m0 = m == -INFINITY ? 0.f : m, sl2 = a.scale_log2;
-  for (int dt = wave; dt < D / 32; dt += 4) {
-    float l = 0.f;
-    float4 o[4];
+  if (desc.tile * M + rg * 32 >= TG) return;
+  const float sl2 = a.scale_log2;
+  float m = -INFINITY, l = 0.f;
+  float4 o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < parts; ++p) {
-      const int64_t slot = slot_of(p);
-      const float2 x = ml[slot * M];
-      const float f = __builtin_amdgcn_exp2f((x.x - m0) * sl2);
-      l += x.y * f;
+  for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = ps; p0 < parts; p0 += PS * kJoin) {
+    float2 x[kJoin];
+    float4 v[kJoin][4];
+    bool has[kJoin];
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      // past the last and runs without a step of the tile: loaded, not used
+      const int p = min(p0 + PS * k, parts - 1);
+      has[k] = p0 + PS * k < parts && paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
+      const int64_t slot = p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p);
+      x[k] = a.ws_ml[slot * M + rg * 32 + ln];
       const float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8) + 4 * dt) * 64 + lane;
 #pragma unroll
+      for (int i = 0; i < 4; ++i) v[k][i] = wo[i * 64];
+      if (!has[k]) x[k] = make_float2(-INFINITY, 0.f);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) m_new = fmaxf(m_new, x[k].x);
+    const float m0 = m_new == -INFINITY ? 0.f : m_new;
+    const float fa = __builtin_amdgcn_exp2f((m - m0) * sl2);
+    m = m_new;
+    l *= fa;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(o[i].x * fa, o[i].y * fa, o[i].z * fa, o[i].w * fa);
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      if (!has[k]) continue;
+      const float f = __builtin_amdgcn_exp2f((x[k].x - m0) * sl2);
+      l += x[k].y * f;
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 v = wo[i * 64];
-        o[i].x += v.x * f;
-        o[i].y += v.y * f;
-        o[i].z += v.z * f;
-        o[i].w += v.w * f;
+        o[i].x += v[k][i].x * f;
+        o[i].y += v[k][i].y * f;
+        o[i].z += v[k][i].z * f;
+        o[i].w += v[k][i].w * f;
       }
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    const int h = desc.y * G + g;
-    T* orow = static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt + 4 * lh;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const T4 v = {(T)(o[i].x * inv), (T)(o[i].y * inv), (T)(o[i].z * inv), (T)(o[i].w * inv)};
-      *reinterpret_cast<T4*>(orow + 8 * i) = v;
-    }
-    if (a.lse != nullptr && dt == 0 && lh == 0)
-      a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] = l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
   }
+  if constexpr (PS > 1) {
+    jml[(ps * DT + dt) * 64 + lane] = make_float2(m, l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) jo[((ps * DT + dt) * 4 + i) * 64 + lane] = o[i];
+    __syncthreads();
+    // wave (dt, ps) takes the lane's float4 ps of the d tile
+    static_assert(PS == 1 || PS == 4, "a float4 to every wave");
+    m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < PS; ++k) m = fmaxf(m, jml[(k * DT + dt) * 64 + lane].x);
+    const float m0 = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < PS; ++k) {
+      const float2 ml = jml[(k * DT + dt) * 64 + lane];
+      const float f = __builtin_amdgcn_exp2f((ml.x - m0) * sl2);
+      const float4 v = jo[((k * DT + dt) * 4 + ps) * 64 + lane];
+      l += ml.y * f;
+      r.x += v.x * f;
+      r.y += v.y * f;
+      r.z += v.z * f;
+      r.w += v.w * f;
+    }
+    o[0] = r;
+  }
+  const int row = desc.tile * M + rg * 32 + ln;
+  if (row >= TG) return;
+  const int t = (int)fdiv((uint32_t)row, a.cut.by_group), h = desc.kvh * G + (row - t * G);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* orow = static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt + 4 * lh;
+#pragma unroll
+  for (int i = 0; i < (PS > 1 ? 1 : 4); ++i) {
+    const T4 v = {(T)(o[i].x * inv), (T)(o[i].y * inv), (T)(o[i].z * inv), (T)(o[i].w * inv)};
+    *reinterpret_cast<T4*>(orow + 8 * (PS > 1 ? ps : i)) = v;
+  }
+  if (a.lse != nullptr && dt == 0 && ps == 0 && lh == 0)
+    a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] = l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
 }
 
 struct Sizes {
@@ -574,7 +803,7 @@ inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv
   const int m = s.few_rows ? 32 : 128;
   s.o = align256((size_t)2 * s.groups * m * head_dim * 4);
   s.ml = align256((size_t)2 * s.groups * m * 8);
-  s.desc = align256((size_t)s.groups * 16);
+  s.desc = align256((size_t)s.groups * sizeof(Args::Desc));
   return s;
 }
 
@@ -603,7 +832,7 @@ template <typename T, int D, int S, int RG> int launch(const Args& a, hipStream_
     attr_set.fetch_or(bit, std::memory_order_acq_rel);
   }
   hipLaunchKernelGGL((varlen_kernel<T, D, S, RG>), dim3((unsigned)a.groups), dim3(C::kWaves * 64), C::kLds, s, a);
-  hipLaunchKernelGGL((combine_kernel<T, D, RG>), dim3((unsigned)a.groups, RG), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((combine_kernel<T, D, RG>), dim3((unsigned)a.groups, RG), dim3(join_split<RG>() * D * 2), 0, s, a);
   return hipGetLastError() == hipSuccess ? TSFA_OK : TSFA_ERR_LAUNCH;
 }
 
@@ -640,8 +869,9 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
     if (p[2] != 1 || p[0] % 8 != 0 || p[1] % 8 != 0) return TSFA_ERR_UNSUPPORTED;
   for (int i = 0; i < 4; ++i)
     if (cache_strides[i] % 8 != 0) return TSFA_ERR_UNSUPPORTED;
-  // a lane's row offset within a page is an unsigned 32-bit byte count
-  if (cache_strides[4] != 1 || cache_strides[2] < 0 || cache_strides[2] > ((int64_t)1 << 26)) return TSFA_ERR_UNSUPPORTED;
+  // a lane's offset from its load's first row is an unsigned 32-bit byte count
+  if (cache_strides[4] != 1 || cache_strides[2] < head_dim || cache_strides[2] > ((int64_t)1 << 26))
+    return TSFA_ERR_UNSUPPORTED;
   if (batch == 0 || total_q == 0) return TSFA_OK;
   for (const void* p : {q, kv_cache, (const void*)o}) {
     if (p == nullptr) return TSFA_ERR_INVALID_ARGUMENT;
@@ -665,11 +895,8 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
   a.mask_n = mask_n;
   a.seqs = make_seqs(q_indptr, kv_lens, kv_indptr, kv_indices, n_indices, page_table_stride, page_table_width, n_pages,
                      page_size, batch, total_q);
-  a.cut.rows = sz.few_rows ? 32 : 128;
-  a.cut.keys = sz.few_rows ? 128 : 64;
-  a.cut.group = num_heads / num_kv_heads;
-  a.cut.num_kv_heads = num_kv_heads;
-  a.cut.causal = mask == nullptr;
+  a.cut = paged::make_cut(sz.few_rows ? 32 : 128, sz.few_rows ? 128 : 64, num_heads / num_kv_heads, num_kv_heads,
+                          mask == nullptr);
   a.sqn = q_strides[0], a.sqh = q_strides[1];
   a.son = o_strides[0], a.soh = o_strides[1];
   a.cp = cache_strides[0], a.cs = cache_strides[1], a.cr = cache_strides[2], a.ch = cache_strides[3];
@@ -681,7 +908,7 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
   char* ws = static_cast<char*>(workspace);
   a.ws_o = reinterpret_cast<float4*>(ws);
   a.ws_ml = reinterpret_cast<float2*>(ws + sz.o);
-  a.ws_desc = reinterpret_cast<int4*>(ws + sz.o + sz.ml);
+  a.ws_desc = reinterpret_cast<varlen::Args::Desc*>(ws + sz.o + sz.ml);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == TSFA_DTYPE_BF16) {
     if (head_dim == 128) return sz.few_rows ? varlen::launch<__bf16, 128, 4, 1>(a, s) : varlen::launch<__bf16, 128, 2, 4>(a, s);

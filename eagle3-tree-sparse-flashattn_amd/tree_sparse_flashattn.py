@@ -811,7 +811,9 @@ def _varlen_lists(q_indptr, kv_lens, kv_indices, kv_indptr, page_size):
     if kv_indptr is not None:
         if kv_indptr.dim() != 1 or kv_indptr.numel() != batch + 1:
             raise ValueError(f"kv_indptr must be int32 [{batch + 1}]")
-        return batch, kv_indices.contiguous().view(-1), 0, 0
+        if kv_indices.dim() != 1:
+            raise ValueError("kv_indices must be a flat int32 list with kv_indptr")
+        return batch, kv_indices.contiguous(), 0, 0
     if kv_indices.dim() != 2 or kv_indices.shape[0] != batch:
         raise ValueError(f"a dense page table must be [{batch}, pages_per_seq] int32")
     if kv_indices.stride(1) != 1 or kv_indices.stride(0) < kv_indices.shape[1]:
@@ -836,19 +838,15 @@ def _same_device(dev, **tensors) -> None:
             raise ValueError(f"{name} must be on {dev}")
 
 
-def _run_on(dev, name: str, launch) -> None:
+def _run_on(dev, name: str, fn, args) -> None:
     # the device guard only when the tensors are not on the current device (~1.2 us)
     if dev.index == torch.cuda.current_device():
-        st = launch(_lib.stream_handle(dev))
+        st = fn(*args, _lib.stream_handle(dev))
     else:
         with torch.cuda.device(dev):
-            st = launch(_lib.stream_handle(dev))
-    _lib.check(name, st)
-
-
-def _packed_heads(name: str, t: torch.Tensor, tokens: int, head_dim: int) -> None:
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != head_dim:
-        raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}], got {tuple(t.shape)}")
+            st = fn(*args, _lib.stream_handle(dev))
+    if st != _lib.TSFA_OK:
+        _lib.check(name, st)
 
 
 def append_paged_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
@@ -878,13 +876,63 @@ def append_paged_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache:
     tokens must not share a place.  No host synchronisation; nothing about the
     lengths is checked on the host.
     """
+    # a geometry that ran as given (no copies) skips the checks its first call
+    # made; everything they look at but the pointers is in the key
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), kv_cache.shape, kv_cache.stride(),
+           kv_indices.shape, kv_indices.stride(), positions.shape, positions.stride(), positions.dtype, inv_freq.shape,
+           inv_freq.stride(), inv_freq.dtype, q_indptr.shape, q_indptr.stride(), kv_lens.shape, kv_lens.stride(),
+           None if kv_indptr is None else (kv_indptr.shape, kv_indptr.stride(), kv_indptr.dtype,
+                                           kv_indptr.get_device()),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device(), out.data_ptr() & 15),
+           q.dtype, k.dtype, v.dtype, kv_cache.dtype, kv_indices.dtype, q_indptr.dtype, kv_lens.dtype, q.get_device(),
+           k.get_device(), v.get_device(), kv_cache.get_device(), kv_indices.get_device(), positions.get_device(),
+           inv_freq.get_device(), q_indptr.get_device(), kv_lens.get_device(),
+           (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15, kv_layout, interleaved, attention_scaling)
+    call = _APPEND_CALLS.get(key)
+    if call is None:
+        call, as_given, (q, k, v, kv_indices, positions, inv_freq, q_indptr, kv_lens, kv_indptr) = _append_plan(
+            q, k, v, kv_cache, kv_indices, positions, inv_freq, q_indptr, kv_lens, kv_indptr, kv_layout, interleaved,
+            attention_scaling, out)
+        if as_given:
+            _remember(_APPEND_CALLS, key, call)
+    dev, rotation, lists, tail, copy_out = call
+    target = torch.empty_like(q) if out is None else out
+    dst = target.contiguous() if copy_out else target
+    fn = _lib.load().tsfa_append_paged_kv
+    ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), dst.data_ptr(), kv_cache.data_ptr(), positions.data_ptr(),
+            rotation[0], inv_freq.data_ptr(), *rotation[1:], q_indptr.data_ptr(), kv_lens.data_ptr(),
+            0 if kv_indptr is None else kv_indptr.data_ptr(), kv_indices.data_ptr(), *lists,
+            *tail)
+    _run_on(dev, "append_paged_kv", fn, ptrs)
+    if copy_out:
+        target.copy_(dst)
+    return target
+
+
+# launch arguments of geometries already checked, by everything the checks
+# look at; the plans under other switches do not differ
+_APPEND_CALLS: dict = {}
+_VARLEN_CALLS: dict = {}
+_SELECT_CALLS: dict = {}
+
+
+def _remember(calls: dict, key, value) -> None:
+    if len(calls) >= 64:
+        calls.clear()
+    calls[key] = value
+
+
+def _append_plan(q, k, v, kv_cache, kv_indices, positions, inv_freq, q_indptr, kv_lens, kv_indptr, kv_layout,
+                 interleaved, attention_scaling, out):
+    """Checks and launch arguments of append_paged_kv, whether its operands are read in place, and those operands."""
+    given = (q, k, v, kv_indices, positions, inv_freq, q_indptr, kv_lens, kv_indptr)
     n_pages, page_size, n_kv_heads, head_dim, cache_strides = _paged_pool(kv_cache, kv_layout)
     if q.dim() != 3:
         raise ValueError(f"q must be [N, Hq, D], got {tuple(q.shape)}")
     n, n_heads = q.shape[0], q.shape[1]
-    _packed_heads("q", q, n, head_dim)
-    _packed_heads("k", k, n, head_dim)
-    _packed_heads("v", v, n, head_dim)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3 or t.shape[0] != n or t.shape[2] != head_dim:
+            raise ValueError(f"{name} must be [{n}, heads, {head_dim}], got {tuple(t.shape)}")
     if k.shape[1] != n_kv_heads or v.shape[1] != n_kv_heads:
         raise ValueError(f"k and v must have the cache's {n_kv_heads} heads")
     if out is not None and tuple(out.shape) != tuple(q.shape):
@@ -902,23 +950,20 @@ def append_paged_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache:
     dev = q.device
     _same_device(dev, q=q, k=k, v=v, kv_cache=kv_cache, kv_indices=kv_indices, kv_indptr=kv_indptr, q_indptr=q_indptr,
                  kv_lens=kv_lens, positions=positions, inv_freq=inv_freq, out=out)
-    qc, k, v = _row_contig(q), _row_contig(k), _row_contig(v)
-    target = torch.empty_like(qc) if out is None else out
-    dst = target if _layout_ok(target) else target.contiguous()
-    lib = _lib.load()
-    args = (batch, n, n_heads, n_kv_heads, head_dim, dt)
+    q, k, v = _row_contig(q), _row_contig(k), _row_contig(v)
     q_indptr, kv_lens, positions, inv_freq = (t.contiguous() for t in (q_indptr, kv_lens, positions, inv_freq))
     kv_indptr = None if kv_indptr is None else kv_indptr.contiguous()
-    _run_on(dev, "append_paged_kv", lambda stream: lib.tsfa_append_paged_kv(
-        qc.data_ptr(), k.data_ptr(), v.data_ptr(), dst.data_ptr(), kv_cache.data_ptr(), positions.data_ptr(),
-        int(positions.dtype == torch.int64), inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved),
-        float(attention_scaling), q_indptr.data_ptr(), kv_lens.data_ptr(), _lib.ptr(kv_indptr), kv_indices.data_ptr(),
-        _table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size,
-        _lib.i64_array((*qc.stride(), *k.stride(), *v.stride(), *dst.stride())), _lib.i64_array(cache_strides), *args,
-        stream))
-    if dst is not target:
-        target.copy_(dst)
-    return target
+    copy_out = out is not None and not _layout_ok(out)
+    dst = torch.empty_like(q) if out is None else out.contiguous() if copy_out else out
+    if not _layout_ok(dst):  # what empty_like makes of q's strides
+        q = q.contiguous()
+        dst = q
+    strides = _lib.i64_array((*q.stride(), *k.stride(), *v.stride(), *dst.stride()))
+    rotation = (int(positions.dtype == torch.int64), 2 * inv_freq.numel(), int(interleaved), float(attention_scaling))
+    lists = (_table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size)
+    tail = (strides, _lib.i64_array(cache_strides), batch, n, n_heads, n_kv_heads, head_dim, dt)
+    operands = (q, k, v, kv_indices, positions, inv_freq, q_indptr, kv_lens, kv_indptr)
+    return (dev, rotation, lists, tail, copy_out), all(x is y for x, y in zip(given, operands)), operands
 
 
 def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tensor, kv_indices: torch.Tensor,
@@ -948,6 +993,42 @@ def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tens
     synchronisation; page ids outside the pool are clamped (wrong O, never an
     invalid read).
     """
+    key = (q.shape, q.stride(), kv_cache.shape, kv_cache.stride(), kv_indices.shape, kv_indices.stride(),
+           q_indptr.shape, q_indptr.stride(), kv_lens.shape, kv_lens.stride(),
+           None if kv_indptr is None else (kv_indptr.shape, kv_indptr.stride(), kv_indptr.dtype,
+                                           kv_indptr.get_device()),
+           None if tree_mask is None else (tree_mask.shape, tree_mask.stride(), tree_mask.dtype,
+                                           tree_mask.get_device()),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device(), out.data_ptr() & 15),
+           q.dtype, kv_cache.dtype, kv_indices.dtype, q_indptr.dtype, kv_lens.dtype, q.get_device(),
+           kv_cache.get_device(), kv_indices.get_device(), q_indptr.get_device(), kv_lens.get_device(),
+           q.data_ptr() & 15, kv_layout, sm_scale)
+    call = _VARLEN_CALLS.get(key)
+    mask = tree_mask
+    if call is None:
+        call, as_given, (q, kv_indices, mask, q_indptr, kv_lens, kv_indptr) = _varlen_plan(
+            q, kv_cache, kv_indices, tree_mask, q_indptr, kv_lens, kv_indptr, kv_layout, sm_scale, out)
+        if as_given:
+            _remember(_VARLEN_CALLS, key, call)
+    dev, mask_args, lists, tail, ws_bytes, copy_out = call
+    target = torch.empty_like(q) if out is None else out
+    dst = target.contiguous() if copy_out else target
+    ws = _workspace(workspace, ws_bytes, dev)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    fn = _lib.load().tsfa_fwd_paged_varlen
+    ptrs = (q.data_ptr(), kv_cache.data_ptr(), dst.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            0 if mask is None else mask.data_ptr(), *mask_args, q_indptr.data_ptr(), kv_lens.data_ptr(),
+            0 if kv_indptr is None else kv_indptr.data_ptr(), kv_indices.data_ptr(), *lists, *tail, ws.data_ptr(),
+            ws_bytes)
+    _run_on(dev, "tree_sparse_attention_fwd_paged_varlen", fn, ptrs)
+    if copy_out:
+        target.copy_(dst)
+    return (target, lse) if return_lse else target
+
+
+def _varlen_plan(q, kv_cache, kv_indices, tree_mask, q_indptr, kv_lens, kv_indptr, kv_layout, sm_scale, out):
+    """Checks and launch arguments of the varlen attention, whether its operands are read in place, and those."""
+    given = (q, kv_indices, tree_mask, q_indptr, kv_lens, kv_indptr)
     n_pages, page_size, n_kv_heads, head_dim, cache_strides = _paged_pool(kv_cache, kv_layout)
     if q.dim() != 3 or q.shape[2] != head_dim:
         raise ValueError(f"q must be [N, Hq, {head_dim}], got {tuple(q.shape)}")
@@ -957,8 +1038,7 @@ def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tens
     if out is not None and tuple(out.shape) != tuple(q.shape):
         raise ValueError(f"out shape {tuple(out.shape)} != q shape {tuple(q.shape)}")
     batch, kv_indices, pt_stride, pt_width = _varlen_lists(q_indptr, kv_lens, kv_indices, kv_indptr, page_size)
-    mask = None
-    mask_seq = mask_row = mask_n = 0
+    mask, mask_args = None, (0, 0, 0)
     if tree_mask is not None:
         if tree_mask.dim() not in (2, 3) or tree_mask.shape[-1] != tree_mask.shape[-2] or tree_mask.shape[-1] < 1:
             raise ValueError(f"tree_mask must be [T, T] or [{batch}, T, T], got {tuple(tree_mask.shape)}")
@@ -967,35 +1047,28 @@ def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tens
         mask = tree_mask if tree_mask.dtype == torch.bool else tree_mask != 0
         if mask.stride(-1) != 1 or min(mask.stride()) < 0:
             mask = mask.contiguous()
-        mask_n, mask_row = mask.shape[-1], mask.stride(-2)
-        mask_seq = mask.stride(0) if mask.dim() == 3 else 0
+        mask_args = (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2), mask.shape[-1])
     if q.dtype != kv_cache.dtype or (out is not None and out.dtype != q.dtype):
         raise NotImplementedError("q, kv_cache and out must share one dtype")
     dt = _lib.dtype_code(q.dtype)
     dev = q.device
     _same_device(dev, q=q, kv_cache=kv_cache, kv_indices=kv_indices, kv_indptr=kv_indptr, q_indptr=q_indptr,
                  kv_lens=kv_lens, tree_mask=mask, out=out)
-    qc = _row_contig(q)
-    target = torch.empty_like(qc) if out is None else out
-    dst = target if _layout_ok(target) else target.contiguous()
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(head_dim)
-    lib = _lib.load()
-    args = (batch, n, n_heads, n_kv_heads, head_dim, dt)
-    ws_bytes = _varlen_workspace_bytes(dev, args)
-    ws = _workspace(workspace, ws_bytes, dev)
-    lse = torch.empty((n, n_heads), dtype=torch.float32, device=dev) if return_lse else None
+    q = _row_contig(q)
     q_indptr, kv_lens = q_indptr.contiguous(), kv_lens.contiguous()
     kv_indptr = None if kv_indptr is None else kv_indptr.contiguous()
-    _run_on(dev, "tree_sparse_attention_fwd_paged_varlen", lambda stream: lib.tsfa_fwd_paged_varlen(
-        qc.data_ptr(), kv_cache.data_ptr(), dst.data_ptr(), _lib.ptr(lse), _lib.ptr(mask), mask_seq, mask_row, mask_n,
-        q_indptr.data_ptr(), kv_lens.data_ptr(), _lib.ptr(kv_indptr), kv_indices.data_ptr(),
-        _table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size, _lib.i64_array(qc.stride()),
-        _lib.i64_array(cache_strides), _lib.i64_array(dst.stride()), float(sm_scale), *args, ws.data_ptr(), ws_bytes,
-        stream))
-    if dst is not target:
-        target.copy_(dst)
-    return (target, lse) if return_lse else target
+    copy_out = out is not None and not _layout_ok(out)
+    dst = torch.empty_like(q) if out is None else out.contiguous() if copy_out else out
+    if not _layout_ok(dst):  # what empty_like makes of q's strides
+        q = q.contiguous()
+        dst = q
+    shape = (batch, n, n_heads, n_kv_heads, head_dim, dt)
+    lists = (_table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size)
+    tail = (_lib.i64_array(q.stride()), _lib.i64_array(cache_strides), _lib.i64_array(dst.stride()),
+            float(1.0 / math.sqrt(head_dim) if sm_scale is None else sm_scale), *shape)
+    operands = (q, kv_indices, mask, q_indptr, kv_lens, kv_indptr)
+    return ((dev, mask_args, lists, tail, _varlen_workspace_bytes(dev, shape), copy_out),
+            all(x is y for x, y in zip(given, operands)), operands)
 
 
 def _varlen_workspace_bytes(dev, args) -> int:
@@ -1042,6 +1115,30 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
     A draft's tree grows by ``parents``: continuation j of this step is a child
     of continuation parents[b, j] of the step before.
     """
+    key = (logits.shape, logits.stride(), logits.dtype, logits.get_device(), scores.shape, scores.stride(),
+           scores.dtype, scores.get_device(), k,
+           tuple([(t.shape, t.stride(), t.dtype, t.get_device()) for t in states]))
+    call = _SELECT_CALLS.get(key)
+    src = states
+    if call is None:
+        call, logits, src = _select_plan(logits, scores, k, states)
+        if all(x is y for x, y in zip(src, states)) and logits.stride() == key[1]:
+            _remember(_SELECT_CALLS, key, call)
+    dev, strides, shape, row_bytes, pointers, ws_bytes = call
+    batch = shape[0]
+    tokens, parents = torch.empty((2, batch, k), dtype=torch.int64, device=dev).unbind(0)
+    best = torch.empty((batch, k), dtype=torch.float32, device=dev)
+    dst = tuple([torch.empty((batch, k, *t.shape[2:]), dtype=t.dtype, device=dev) for t in src])
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=dev)
+    _run_on(dev, "beam_select", _lib.load().tsfa_beam_select,
+            (logits.data_ptr(), strides[0], strides[1], scores.data_ptr(), strides[2], strides[3], *shape,
+             tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), pointers(*[t.data_ptr() for t in src]),
+             pointers(*[t.data_ptr() for t in dst]), row_bytes, len(src), ws.data_ptr(), ws_bytes))
+    return BeamSelection(tokens, parents, best, dst)
+
+
+def _select_plan(logits, scores, k, states):
+    """Checks and launch arguments of beam_select, and its operands as they are read."""
     if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]):
         raise ValueError(f"logits must be [B, W, V] and scores [B, W], got {tuple(logits.shape)} and "
                          f"{tuple(scores.shape)}")
@@ -1059,20 +1156,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
         _same_device(dev, **{f"states[{i}]": t})
     if logits.stride(2) != 1:
         logits = logits.contiguous()
-    lib = _lib.load()
-    new = dict(device=dev, dtype=torch.int64)
-    tokens, parents = torch.empty((batch, k), **new), torch.empty((batch, k), **new)
-    best = torch.empty((batch, k), dtype=torch.float32, device=dev)
-    src = [t.contiguous() for t in states]
-    dst = [torch.empty((batch, k, *t.shape[2:]), dtype=t.dtype, device=dev) for t in src]
-    n = len(src)
-    pointers = ctypes.c_void_p * max(n, 1)
-    row_bytes = [t[0, 0].numel() * t.element_size() if t.numel() else 0 for t in src]
-    ws_bytes = int(lib.tsfa_beam_select_workspace_bytes(batch, beams, vocab, k))
-    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=dev)
-    _run_on(dev, "beam_select", lambda stream: lib.tsfa_beam_select(
-        logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), scores.stride(0), scores.stride(1),
-        batch, beams, vocab, k, dt, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(),
-        pointers(*(t.data_ptr() for t in src)), pointers(*(t.data_ptr() for t in dst)), _lib.i64_array(row_bytes), n,
-        ws.data_ptr(), ws_bytes, stream))
-    return BeamSelection(tokens, parents, best, tuple(dst))
+    src = tuple([t.contiguous() for t in states])
+    row_bytes = _lib.i64_array([t[0, 0].numel() * t.element_size() if t.numel() else 0 for t in src])
+    ws_bytes = int(_lib.load().tsfa_beam_select_workspace_bytes(batch, beams, vocab, k))
+    strides = (logits.stride(0), logits.stride(1), scores.stride(0), scores.stride(1))
+    call = (dev, strides, (batch, beams, vocab, k, dt), row_bytes, ctypes.c_void_p * max(len(src), 1), ws_bytes)
+    return call, logits, src

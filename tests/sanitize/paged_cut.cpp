@@ -50,13 +50,8 @@ int main() {
     }
     Seqs s = make_seqs(qi.data(), kl.data(), dense ? nullptr : pi.data(), indices.data(), (int64_t)indices.size(),
                        width, width, 4, 1 << page_shift, batch, total_q);
-    Cut c;
     const int rg = 1 << pick(0, 3), streams = 1 << pick(0, 2);
-    c.rows = 32 * rg;
-    c.keys = 32 * streams;
-    c.group = pick(1, 9);
-    c.num_kv_heads = pick(1, 4);
-    c.causal = pick(0, 1);
+    const Cut c = make_cut(32 * rg, 32 * streams, pick(1, 9), pick(1, 4), pick(0, 1));
     const int groups = pick(0, 1) ? 256 : pick(1, 40);
 
     int64_t total = 0;
@@ -65,60 +60,79 @@ int main() {
       CHECK(q.q0 >= 0 && q.q_len >= 0 && q.q0 + q.q_len <= total_q && q.kv_len >= 0 && q.prefix >= 0);
       CHECK(q.list >= 0 && q.pages >= 0 && q.list + q.pages <= (int64_t)indices.size());
       CHECK(((int64_t)q.pages << page_shift) >= q.kv_len && q.prefix <= q.kv_len);
-      total += head_steps(c, q) * c.num_kv_heads;
+      total += head_length(c, q) * c.num_kv_heads;
+      int64_t sum = 0;
+      for (int r = 0; r < cut_tiles(c, q); ++r) {
+        CHECK(tiles_length(c, q, r) == sum);
+        const int64_t len = tile_first(c, q) + tile_more(c) * r;
+        CHECK(len >= tile_steps(c, q, r) * c.unit);  // steps start a step's length apart
+        sum += len;
+      }
+      CHECK(head_length(c, q) == sum);
     }
-    if (total == 0 || total > 400000) continue;
-    const int64_t per = (total + groups - 1) / groups;
-    const int used = (int)((total + per - 1) / per);
-    CHECK(used <= groups);
+    if (total == 0 || total / c.unit > 400000) continue;
+    const int64_t per = run_length(c, total, groups);
     std::map<std::tuple<int, int, int>, std::vector<std::tuple<int, int, int>>> parts;  // tile -> (run, s0, s1)
-    for (int run = 0; run < used; ++run) {
-      int64_t at = run * per;
+    CHECK(per * groups >= total);
+    for (int run = 0; run < groups; ++run) {
+      const int64_t at = run * per;
+      if (at >= total) break;
       const int64_t end = std::min(at + per, total);
-      CHECK(at < end);
       int b = 0;
       int64_t before = 0;
       for (;; ++b) {
         CHECK(b < batch);
-        const int64_t n = head_steps(c, seq_of(s, b)) * c.num_kv_heads;
+        const int64_t n = head_length(c, seq_of(s, b)) * c.num_kv_heads;
         if (before + n > at) break;
         before += n;
       }
-      Place p = place_in_seq(c, seq_of(s, b), b, at - before);
-      for (;;) {
-        const int n = tile_steps(c, p.seq, p.tile), s0 = p.step;
-        CHECK(p.tile < cut_tiles(c, p.seq) && p.kvh < c.num_kv_heads && s0 < n);
-        const int s1 = (int)(end - at < n - s0 ? s0 + (end - at) : n);
-        parts[{p.b, p.kvh, p.tile}].push_back({run, s0, s1});
-        for (int c0 = s0; c0 < s1 && p.seq.kv_len > 0;) {
-          const Chunk k = chunk_of(p.seq, page_shift, streams, c0, s1, !c.causal);
+      Seq q = seq_of(s, b);
+      Place p = place_in_seq(c, q, at - before);
+      int64_t left = end - (at - p.from);
+      bool more = true;
+      auto next = [&]() {
+        do {
+          if (++b >= batch) return false;
+          q = seq_of(s, b);
+        } while (q.q_len == 0);
+        return true;
+      };
+      if (p.kvh == c.num_kv_heads) {
+        p.kvh = 0;
+        more = next();
+      }
+      while (more) {
+        const int n = tile_steps(c, q, p.tile), s0 = p.step;
+        CHECK(p.tile < cut_tiles(c, q) && p.kvh < c.num_kv_heads && s0 < n);
+        const int s1 = steps_before(c, left, n);
+        if (s0 >= s1) break;
+        parts[{b, p.kvh, p.tile}].push_back({run, s0, s1});
+        for (int c0 = s0; c0 < s1 && q.kv_len > 0;) {
+          const Chunk k = chunk_of(q, page_shift, streams, c0, s1, !c.causal);
           CHECK(k.end > c0 && k.end <= s1 && k.first_page >= 0 && k.ids >= 1 && k.ids <= kTableIds);
-          CHECK(k.first_page + k.ids <= p.seq.pages);
+          CHECK(k.first_page + k.ids <= q.pages);
           if (!c.causal) CHECK(k.end * streams - k.tree_unit <= kTreeUnits);
           for (int u = c0 * streams; u < k.end * streams; ++u) {
-            if ((u + 1) * 32 > p.seq.prefix) CHECK(u >= k.tree_unit);
+            if ((u + 1) * 32 > q.prefix) CHECK(u >= k.tree_unit);
             for (int rpl : {4, 8})
               for (int kb = 0; kb < 32; kb += rpl) {
-                const int blk = load_block(u * 32 + kb, rpl, p.seq.kv_len);
-                CHECK(blk >= 0 && blk < p.seq.kv_len);
+                const int blk = load_block(u * 32 + kb, rpl, q.kv_len);
+                CHECK(blk >= 0 && blk < q.kv_len);
                 const int id = (blk >> page_shift) - k.first_page;
                 CHECK(id >= 0 && id < k.ids);
               }
           }
           c0 = k.end;
         }
-        at += s1 - s0;
-        if (at >= end) break;
+        if (s1 < n) break;
+        left -= tile_first(c, q) + tile_more(c) * p.tile;
+        if (left <= 0) break;
         p.step = 0;
-        if (++p.tile == cut_tiles(c, p.seq)) {
+        if (++p.tile == cut_tiles(c, q)) {
           p.tile = 0;
           if (++p.kvh == c.num_kv_heads) {
             p.kvh = 0;
-            do {
-              ++p.b;
-              CHECK(p.b < batch);
-              p.seq = seq_of(s, p.b);
-            } while (cut_tiles(c, p.seq) == 0);
+            more = next();
           }
         }
       }
@@ -134,13 +148,22 @@ int main() {
           int upto = 0;
           for (size_t i = 0; i < v.size(); ++i) {
             auto [run, s0, s1] = v[i];
-            CHECK(s0 == upto && s1 > s0 && run == std::get<0>(v[0]) + (int)i);
+            CHECK(s0 == upto && s1 > s0 && run >= std::get<0>(v[0]) + (int)i);
             upto = s1;
           }
           CHECK(upto == n);
+          // the runs between the first and the last part's that hold a part are those run_has_step names
+          size_t held = 0;
+          for (int run = std::get<0>(v.front()); run <= std::get<0>(v.back()); ++run)
+            if (run_has_step(c, run * per, per, line)) {
+              CHECK(held < v.size() && std::get<0>(v[held]) == run);
+              ++held;
+            }
+          CHECK(held == v.size());
           // the number of parts as the first run writes it for the join
-          if (v.size() > 1) CHECK((int)((line + n - 1) / per - std::get<0>(v[0])) + 1 == (int)v.size());
-          line += n;
+          if (v.size() > 1)
+            CHECK((int)udiv(line + (n - 1) * c.unit, per, 1.0 / per) == std::get<0>(v.back()));
+          line += tile_first(c, q) + tile_more(c) * t;
         }
     }
     CHECK(line == total);

@@ -17,7 +17,8 @@ GXX = shutil.which("g++")
 def test_every_step_belongs_to_one_run(tmp_path):
     exe = tmp_path / "paged_cut"
     subprocess.run([GXX, "-std=c++17", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-g", "-O1",
-                    f"-I{CSRC}", str(ROOT / "tests" / "sanitize" / "paged_cut.cpp"), "-o", str(exe)],
+                    f"-I{CSRC}", str(ROOT / "tests" / "sanitize" / "paged_cut.cpp"),
+                    str(CSRC / "tsfa_plan.cpp"), "-o", str(exe)],
                    check=True, capture_output=True, text=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300,
                          env={**os.environ, "ASAN_OPTIONS": "detect_leaks=1", "UBSAN_OPTIONS": "print_stacktrace=1"})
