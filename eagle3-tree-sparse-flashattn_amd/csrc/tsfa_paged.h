@@ -70,7 +70,9 @@ TSFA_HD inline Seq seq_of(const Seqs& s, int b) {
 // key, prefix + ((r + 1) rows - 1) / group, linear in r on this scale, so the
 // place of a tile is a closed form both ways and no workgroup walks the tiles
 // before its own (a loop over them took tens of microseconds for prompts of
-// 1000 tokens).  Either way steps start a step's length apart at least.
+// 1000 tokens).  Either way steps start a step's length apart at least, and
+// `extra` steps of nothing at a tile's end stand for what starting and ending
+// a tile costs, so that a run of many short tiles has fewer steps.
 struct Cut {
   int rows, keys;           // tile height, keys of a step (powers of two)
   int group, num_kv_heads;  // query heads per kv head; kv heads
@@ -79,9 +81,10 @@ struct Cut {
   FastDiv by_group;
   int64_t unit;             // line length of a step: keys * group
   double inv_unit;
+  int extra;                // steps that a tile's start and end cost
 };
 
-inline Cut make_cut(int rows, int keys, int group, int num_kv_heads, int causal) {
+inline Cut make_cut(int rows, int keys, int group, int num_kv_heads, int causal, int extra) {
   Cut c;
   c.rows = rows;
   c.keys = keys;
@@ -93,6 +96,7 @@ inline Cut make_cut(int rows, int keys, int group, int num_kv_heads, int causal)
   c.by_group = make_fastdiv((uint32_t)group);
   c.unit = (int64_t)keys * group;
   c.inv_unit = 1.0 / (double)c.unit;
+  c.extra = extra;
   return c;
 }
 
@@ -124,8 +128,8 @@ TSFA_HD inline int tile_steps(const Cut& c, const Seq& s, int r) {
 // Line lengths: tile 0 of a sequence and what each further tile adds to it,
 // the first r tiles, and one kv head.
 TSFA_HD inline int64_t tile_first(const Cut& c, const Seq& s) {
-  if (c.causal) return ((int64_t)s.prefix + 1) * c.group + c.rows - 1 + c.unit - 1;
-  return tile_steps(c, s, 0) * c.unit;
+  if (c.causal) return ((int64_t)s.prefix + 1) * c.group + c.rows - 1 + c.unit - 1 + c.extra * c.unit;
+  return (tile_steps(c, s, 0) + c.extra) * c.unit;
 }
 TSFA_HD inline int64_t tile_more(const Cut& c) { return c.causal ? c.rows : 0; }
 TSFA_HD inline int64_t tiles_length(const Cut& c, const Seq& s, int64_t r) {

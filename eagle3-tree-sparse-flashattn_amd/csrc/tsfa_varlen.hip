@@ -93,7 +93,7 @@ __device__ inline void dma_1k(const void* base, uint32_t off, uint32_t lds_in) {
 // N such loads to consecutive LDS KBs from one base: load i reads base +
 // off[i] + i KB (the immediate offset counts for both addresses).
 template <int N> __device__ inline void dma_rows(const void* base, const uint32_t (&off)[N], uint32_t lds_in) {
-  static_assert(N == 2 || N == 4, "16 key rows");
+  static_assert(N == 1 || N == 2 || N == 4, "up to 16 key rows");
   const uint64_t u = reinterpret_cast<uint64_t>(base);
   const uint64_t sbase = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(u >> 32)) << 32) |
                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)u);
@@ -104,6 +104,11 @@ template <int N> __device__ inline void dma_rows(const void* base, const uint32_
                  "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
                  :
                  : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(sbase), "s"(lds)
+                 : "memory", "m0");
+  else if constexpr (N == 1)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off[0]), "s"(sbase), "s"(lds)
                  : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\t"
@@ -206,10 +211,11 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   // two elements' exponent bits, and what carries all-ones exponents into bit 15
   constexpr uint32_t EXP2 = std::is_same<T, __bf16>::value ? 0x7f807f80u : 0x7c007c00u;
   constexpr uint32_t ONE2 = std::is_same<T, __bf16>::value ? 0x00800080u : 0x04000400u;
-  constexpr int GL = 16 / RPL;    // loads of 16 key rows (never more than a page)
-  constexpr int NG = LPW / GL;    // groups of 16 rows a wave moves per unit
+  constexpr int GL = 16 / RPL;             // loads of 16 key rows (never more than a page)
+  constexpr int GW = LPW < GL ? LPW : GL;  // loads of such a group that a wave makes
+  constexpr int NG = LPW / GW;             // groups a wave moves, or shares, per unit
   constexpr bool PIPE = NST >= 4;  // the next unit's scores run under this unit's softmax
-  static_assert(NG >= 1 && LPW % GL == 0 && LPW * (NST - 1) < 64 && NST >= 2, "ring");
+  static_assert(NG >= 1 && LPW % GW == 0 && GL % GW == 0 && LPW * (NST - 1) < 64 && NST >= 2, "ring");
   extern __shared__ __attribute__((aligned(256))) unsigned char smem[];
   int32_t* table = reinterpret_cast<int32_t*>(smem + C::kRing);
   uint32_t* words = reinterpret_cast<uint32_t*>(smem + C::kRing + kTableIds * 4);
@@ -274,14 +280,14 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     if (!next_seq()) return;
   }
 
-  // The wave's share of a unit: groups rg NG .. rg NG + NG - 1 of 16 key rows
-  // (groups 0 and 1 are K's, 2 and 3 V's).  Chunk x of row k lies at chunk x ^
-  // swz(k), and both swizzles have a period that divides 16.
+  // The wave's share of a unit: loads rg LPW .. rg LPW + LPW - 1 of its 4 GL
+  // (groups of 16 key rows, 0 and 1 K's, 2 and 3 V's).  Chunk x of row k lies
+  // at chunk x ^ swz(k), and both swizzles have a period that divides 16.
   const uint32_t ring = lds_addr(smem) + (uint32_t)(st * NST * C::kUnit);
-  uint32_t off_k[GL], off_v[GL];
+  uint32_t off_k[GW], off_v[GW];
 #pragma unroll
-  for (int i = 0; i < GL; ++i) {
-    const int row = i * RPL + lane / CPR;
+  for (int i = 0; i < GW; ++i) {
+    const int row = (rg * LPW % GL + i) * RPL + lane / CPR;
     const uint32_t at_row = (uint32_t)row * (uint32_t)a.cr * 2u - (uint32_t)i * 1024u;
     off_k[i] = at_row + (uint32_t)(((lane % CPR) ^ swz_k<D>(row)) << 4);
     off_v[i] = at_row + (uint32_t)(((lane % CPR) ^ swz_v<D>(row)) << 4);
@@ -346,30 +352,34 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       const int c1 = ck.end, first_page = ck.first_page, ids = ck.ids, ut0 = ck.tree_unit;
       for (int i = tid; i < ids; i += C::kWaves * 64)
         table[i] = min(max(a.seqs.kv_indices[sq.list + first_page + i], 0), a.seqs.n_pages - 1);
-      if (a.mask != nullptr) {
-        for (int i = tid; i < (c1 * S - ut0) * M; i += C::kWaves * 64) {
-          const int row = min(pl.tile * M + i % M, TG - 1);
-          words[i] = word_of((ut0 + i / M) * 32, (int)fdiv((uint32_t)row, cut.by_group));
-        }
-      }
       barrier();
 
       // Unit j of the chunk's stream into stage j % NST.  Units that reach past
       // the last key take their rows load by load, each from a block that holds
       // a key, so that no stale value of the pool enters P V.
       const int n = c1 - c0;
+      // page ids of the next unit to request, read from the table a step ahead
+      int next_id[NG];
+      auto peek = [&](int j) {
+        const int k0 = ((c0 + j) * S + st) * 32;
+#pragma unroll
+        for (int x = 0; x < NG; ++x)
+          next_id[x] = table[min((min(k0 + 16 * ((rg * LPW / GL + x) & 1), kl - 1) >> ps) - first_page, kTableIds - 1)];
+      };
+      peek(0);
       auto issue = [&](int j) {
         const int k0 = ((c0 + j) * S + st) * 32;
         const uint32_t dst = ring + (uint32_t)((j % NST) * C::kUnit);
         if (k0 + 32 <= kl) {
 #pragma unroll
           for (int x = 0; x < NG; ++x) {
-            const int grp = rg * NG + x;
+            const int grp = rg * LPW / GL + x;
             const int key = k0 + 16 * (grp & 1);
-            const int id = __builtin_amdgcn_readfirstlane(table[(key >> ps) - first_page]);
+            const int id = __builtin_amdgcn_readfirstlane(next_id[x]);
             const T* base = hbase + id * a.cp + (grp >= 2 ? a.cs : 0) + (int64_t)(key & ((1 << ps) - 1)) * a.cr;
-            if (grp >= 2) dma_rows<GL>(base, off_v, dst + (uint32_t)grp * (GL * 1024u));
-            else dma_rows<GL>(base, off_k, dst + (uint32_t)grp * (GL * 1024u));
+            const uint32_t to = dst + (uint32_t)(rg * LPW + x * GW) * 1024u;
+            if (grp >= 2) dma_rows<GW>(base, off_v, to);
+            else dma_rows<GW>(base, off_k, to);
           }
         } else {
           for (int x = 0; x < LPW; ++x) {
@@ -385,6 +395,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
             dma_1k(base, (uint32_t)from * (uint32_t)a.cr * 2u + (uint32_t)chunk * 16u, dst + (uint32_t)u * 1024u);
           }
         }
+        peek(j + 1);
       };
 
       // S^T of the unit at kt: lane (ln, lh) element i is key 8 (i / 4) + 4 lh
@@ -414,6 +425,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         return s;
       };
       auto none = [](auto...) {};
+      int issued = 0;
 
       // Unit j, whose scores are in s: online softmax, O^T += V^T P^T.  NEXT: a
       // unit that every row sees whole, unit j + 1's scores (left in s) between
@@ -445,7 +457,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           alpha = need ? __builtin_amdgcn_exp2f((m_run - m_new) * sl2) : 1.f;
           m_run = m_new;
           m_lim = m_new + thr;
-          ms = m_new == -INFINITY ? 0.f : m_new;
+          ms = m_new == -INFINITY ? 0.f : m_new * sl2;
         };
         // P is rounded to the input type for the product with V, which takes
         // 16-bit operands; its row sum takes the unrounded values.  Pinned where
@@ -453,7 +465,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         float psum = 0.f, p[16];
         uint32_t pk[8];
         auto expo = [&](int i) {
-          p[i] = __builtin_amdgcn_exp2f((s[i] - ms) * sl2);
+          p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl2, -ms));
           psum += p[i];
           if (i & 1) {
             pk[i >> 1] = bit_cast<uint32_t>(T2{(T)p[i - 1], (T)p[i]});
@@ -461,7 +473,10 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           }
         };
         if constexpr (NEXT) {
-          const f32x16 sn = scores(smem + (st * NST + (j + 1) % NST) * C::kUnit, stats, [&](int kk) {
+          const f32x16 sn = scores(smem + (st * NST + (j + 1) % NST) * C::kUnit, [&]() {
+            if (issued < n) issue(issued++);
+            stats();
+          }, [&](int kk) {
 #pragma unroll
             for (int i = 16 / KS * kk; i < 16 / KS * (kk + 1); ++i) expo(i);
           });
@@ -542,8 +557,15 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       };
 
       vm_wait<0>();  // the ring's waits count its own loads alone
-      for (int j = 0; j < NST - 1 && j < n; ++j) issue(j);
-      int issued = min(n, NST - 1), j = 0;
+      while (issued < NST - 1 && issued < n) issue(issued++);
+      if (a.mask != nullptr) {
+        // under the first units' way here; the barriers below order them
+        for (int i = tid; i < (c1 * S - ut0) * M; i += C::kWaves * 64) {
+          const int row = min(pl.tile * M + i % M, TG - 1);
+          words[i] = word_of((ut0 + i / M) * 32, (int)fdiv((uint32_t)row, cut.by_group));
+        }
+      }
+      int j = 0;
       wait_units<LPW, NST - 2>(issued - 1);
       barrier();
       f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
@@ -554,7 +576,6 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           // unit j + 1 is there, and every wave is done with unit j - 1
           wait_units<LPW, NST - 3>(issued - 2 - j);
           barrier();
-          if (issued < n) issue(issued++);
           unit(std::true_type{}, j, s);
         }
       }
@@ -578,8 +599,8 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     const bool whole = s0 == 0 && s1 == n_steps;
     float4* jo = reinterpret_cast<float4*>(smem);                              // the streams' O
     float2* jml = reinterpret_cast<float2*>(smem + C::kRing + kTableIds * 4);  // [S][RG][32] (m, l)
-    static_assert(S * RG * 32 * 8 <= C::kWords && S * RG * X * 1024 <= C::kRing, "join");
-    if (lh == 0) jml[(st * RG + rg) * 32 + ln] = make_float2(m_run, l_run);
+    static_assert(S * RG * 32 * 8 <= C::kWords && (S == 1 || S * RG * X * 1024 <= C::kRing), "join");
+    if (S > 1 && lh == 0) jml[(st * RG + rg) * 32 + ln] = make_float2(m_run, l_run);
     float mm = -INFINITY, ll = 0.f, fs[S];
     auto weights = [&]() {
       float2 ml[S];
@@ -613,7 +634,12 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       const int dt = x >> 2, i = x & 3;
       return make_float4(o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]);
     };
-    if constexpr (S == 2) {
+    if constexpr (S == 1) {
+      mm = m_run;
+      ll = l_run;
+#pragma unroll
+      for (int x = 0; x < X; ++x) put(x, o4(x));
+    } else if constexpr (S == 2) {
       // each stream leaves the other's half and finishes its own
       float4* mine = jo + ((st * RG + rg) * XS) * 64 + lane;
       const float4* other = jo + (((1 - st) * RG + rg) * XS) * 64 + lane;
@@ -682,127 +708,148 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   }
 }
 
-// Joins the parts of the tiles that several runs share: block (run, row
-// group), a wave to every d tile and, with few row groups, PS waves that split
-// the parts; kJoin parts loaded at once.
+// Joins the parts of the tiles that several runs share.  Work items are (tile,
+// row group, d tile): every block lists the tiles first (one load of all runs'
+// descriptors) and takes items blockIdx.x, + gridDim.x, ...; its four waves
+// split the parts, kJoin of them loaded at once.  A block per run would leave
+// most of them empty and the others few: 17 us against %JOIN% us for 16 tiles
+// in 14 parts each.
 constexpr int kJoin = 4;
-template <int RG> constexpr int join_split() { return RG == 1 ? 4 : 1; }
+constexpr int kMaxGroups = 1024;
 template <typename T, int D, int RG>
-__global__ __launch_bounds__(join_split<RG>() * D * 2) void combine_kernel(const Args a) {
+__global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   typedef T T4 __attribute__((ext_vector_type(4)));
-  constexpr int DT = D / 32, PS = join_split<RG>(), M = 32 * RG;
-  __shared__ float4 jo[PS > 1 ? PS * DT * 4 * 64 : 1];
-  __shared__ float2 jml[PS > 1 ? PS * DT * 64 : 1];
-  const int run = blockIdx.x, rg = blockIdx.y;
-  const Args::Desc desc = a.ws_desc[run];
-  const int parts = desc.runs;
-  if (parts == 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int DT = D / 32, PS = 4, M = 32 * RG;
+  __shared__ float4 jo[PS * 4 * 64];
+  __shared__ float2 jml[PS * 64];
+  __shared__ short tiles[kMaxGroups];
+  __shared__ int wave_count[kMaxGroups / 64];
+  const int lane = threadIdx.x & 63, ps = threadIdx.x >> 6;
   const int ln = lane & 31, lh = lane >> 5;
-  const int dt = wave % DT, ps = wave / DT;
-  const Seq sq = paged::seq_of(a.seqs, desc.b);
-  const int G = a.cut.group, TG = sq.q_len * G;
-  if (desc.tile * M + rg * 32 >= TG) return;
+  for (int r0 = ps * 64; r0 < a.groups; r0 += 256) {
+    const bool on = r0 + lane < a.groups && a.ws_desc[r0 + lane].runs != 0;
+    const uint64_t set = __ballot(on);
+    if (lane == 0) wave_count[r0 / 64] = __builtin_popcountll(set);
+  }
+  __syncthreads();
+  int n_tiles = 0;
+  for (int w = 0; w * 64 < a.groups; ++w) n_tiles += wave_count[w];
+  const int n_items = n_tiles * RG * DT;
+  if ((int)blockIdx.x >= n_items) return;
+  for (int r0 = ps * 64; r0 < a.groups; r0 += 256) {
+    const bool on = r0 + lane < a.groups && a.ws_desc[r0 + lane].runs != 0;
+    const uint64_t set = __ballot(on);
+    int at = __builtin_popcountll(set & ((1ull << lane) - 1));
+    for (int w = 0; w < r0 / 64; ++w) at += wave_count[w];
+    if (on) tiles[at] = (short)(r0 + lane);
+  }
+  __syncthreads();
   const float sl2 = a.scale_log2;
-  float m = -INFINITY, l = 0.f;
-  float4 o[4];
+  for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    const int run = tiles[item / (RG * DT)], rg = item / DT % RG, dt = item % DT;
+    const Args::Desc desc = a.ws_desc[run];
+    const int parts = desc.runs;
+    const Seq sq = paged::seq_of(a.seqs, desc.b);
+    const int G = a.cut.group, TG = sq.q_len * G;
+    if (desc.tile * M + rg * 32 >= TG) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 o[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = ps; p0 < parts; p0 += PS * kJoin) {
-    float2 x[kJoin];
-    float4 v[kJoin][4];
-    bool has[kJoin];
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = ps; p0 < parts; p0 += PS * kJoin) {
+      float2 x[kJoin];
+      float4 v[kJoin][4];
+      bool has[kJoin];
 #pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      // past the last and runs without a step of the tile: loaded, not used
-      const int p = min(p0 + PS * k, parts - 1);
-      has[k] = p0 + PS * k < parts && paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
-      const int64_t slot = p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p);
-      x[k] = a.ws_ml[slot * M + rg * 32 + ln];
-      const float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8) + 4 * dt) * 64 + lane;
+      for (int k = 0; k < kJoin; ++k) {
+        // past the last and runs without a step of the tile: loaded, not used
+        const int p = min(p0 + PS * k, parts - 1);
+        has[k] = p0 + PS * k < parts && paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
+        const int64_t slot = p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p);
+        x[k] = a.ws_ml[slot * M + rg * 32 + ln];
+        const float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8) + 4 * dt) * 64 + lane;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[k][i] = wo[i * 64];
-      if (!has[k]) x[k] = make_float2(-INFINITY, 0.f);
-    }
-    float m_new = m;
+        for (int i = 0; i < 4; ++i) v[k][i] = wo[i * 64];
+        if (!has[k]) x[k] = make_float2(-INFINITY, 0.f);
+      }
+      float m_new = m;
 #pragma unroll
-    for (int k = 0; k < kJoin; ++k) m_new = fmaxf(m_new, x[k].x);
-    const float m0 = m_new == -INFINITY ? 0.f : m_new;
-    const float fa = __builtin_amdgcn_exp2f((m - m0) * sl2);
-    m = m_new;
-    l *= fa;
+      for (int k = 0; k < kJoin; ++k) m_new = fmaxf(m_new, x[k].x);
+      const float m0 = m_new == -INFINITY ? 0.f : m_new;
+      const float fa = __builtin_amdgcn_exp2f((m - m0) * sl2);
+      m = m_new;
+      l *= fa;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = make_float4(o[i].x * fa, o[i].y * fa, o[i].z * fa, o[i].w * fa);
+      for (int i = 0; i < 4; ++i) o[i] = make_float4(o[i].x * fa, o[i].y * fa, o[i].z * fa, o[i].w * fa);
 #pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      if (!has[k]) continue;
-      const float f = __builtin_amdgcn_exp2f((x[k].x - m0) * sl2);
-      l += x[k].y * f;
+      for (int k = 0; k < kJoin; ++k) {
+        if (!has[k]) continue;
+        const float f = __builtin_amdgcn_exp2f((x[k].x - m0) * sl2);
+        l += x[k].y * f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i].x += v[k][i].x * f;
-        o[i].y += v[k][i].y * f;
-        o[i].z += v[k][i].z * f;
-        o[i].w += v[k][i].w * f;
+        for (int i = 0; i < 4; ++i) {
+          o[i].x += v[k][i].x * f;
+          o[i].y += v[k][i].y * f;
+          o[i].z += v[k][i].z * f;
+          o[i].w += v[k][i].w * f;
+        }
       }
     }
-  }
-  if constexpr (PS > 1) {
-    jml[(ps * DT + dt) * 64 + lane] = make_float2(m, l);
+    jml[ps * 64 + lane] = make_float2(m, l);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) jo[((ps * DT + dt) * 4 + i) * 64 + lane] = o[i];
+    for (int i = 0; i < 4; ++i) jo[(ps * 4 + i) * 64 + lane] = o[i];
     __syncthreads();
-    // wave (dt, ps) takes the lane's float4 ps of the d tile
-    static_assert(PS == 1 || PS == 4, "a float4 to every wave");
+    // wave ps takes the lane's float4 ps
     m = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < PS; ++k) m = fmaxf(m, jml[(k * DT + dt) * 64 + lane].x);
+    for (int k = 0; k < PS; ++k) m = fmaxf(m, jml[k * 64 + lane].x);
     const float m0 = m == -INFINITY ? 0.f : m;
     l = 0.f;
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < PS; ++k) {
-      const float2 ml = jml[(k * DT + dt) * 64 + lane];
+      const float2 ml = jml[k * 64 + lane];
       const float f = __builtin_amdgcn_exp2f((ml.x - m0) * sl2);
-      const float4 v = jo[((k * DT + dt) * 4 + ps) * 64 + lane];
+      const float4 v = jo[(k * 4 + ps) * 64 + lane];
       l += ml.y * f;
       r.x += v.x * f;
       r.y += v.y * f;
       r.z += v.z * f;
       r.w += v.w * f;
     }
-    o[0] = r;
+    const int row = desc.tile * M + rg * 32 + ln;
+    if (row < TG) {
+      const int t = (int)fdiv((uint32_t)row, a.cut.by_group), h = desc.kvh * G + (row - t * G);
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const T4 v = {(T)(r.x * inv), (T)(r.y * inv), (T)(r.z * inv), (T)(r.w * inv)};
+      *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt +
+                             8 * ps + 4 * lh) = v;
+      if (a.lse != nullptr && dt == 0 && ps == 0 && lh == 0)
+        a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] =
+            l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
+    }
+    __syncthreads();  // jo and jml are written again
   }
-  const int row = desc.tile * M + rg * 32 + ln;
-  if (row >= TG) return;
-  const int t = (int)fdiv((uint32_t)row, a.cut.by_group), h = desc.kvh * G + (row - t * G);
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* orow = static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt + 4 * lh;
-#pragma unroll
-  for (int i = 0; i < (PS > 1 ? 1 : 4); ++i) {
-    const T4 v = {(T)(o[i].x * inv), (T)(o[i].y * inv), (T)(o[i].z * inv), (T)(o[i].w * inv)};
-    *reinterpret_cast<T4*>(orow + 8 * (PS > 1 ? ps : i)) = v;
-  }
-  if (a.lse != nullptr && dt == 0 && ps == 0 && lh == 0)
-    a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] = l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
 }
 
 struct Sizes {
-  int groups, few_rows;
+  int groups, rows, streams, extra;
   size_t o, ml, desc;
   size_t total() const { return o + ml + desc; }
 };
 
-// 32-row tiles with four key streams where a sequence has at most 32 rows on
-// average, else 128-row tiles with two.
+// Tiles by the rows (query token x head of a kv head) of a sequence on
+// average: 32 rows and four key streams up to 32 of them (decoding), 256 rows
+// and one stream above 512, else 128 rows and two.
 inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim) {
   Sizes s;
   const int64_t rows = (int64_t)total_q * (num_heads / num_kv_heads);
-  s.few_rows = rows <= (int64_t)32 * batch;
-  s.groups = cus;
-  const int m = s.few_rows ? 32 : 128;
-  s.o = align256((size_t)2 * s.groups * m * head_dim * 4);
-  s.ml = align256((size_t)2 * s.groups * m * 8);
+  s.rows = rows <= (int64_t)32 * batch ? 32 : rows > (int64_t)512 * batch ? 256 : 128;
+  s.streams = s.rows == 32 ? 4 : s.rows == 256 ? 1 : 2;
+  s.extra = s.rows == 32 ? 3 : s.rows == 256 ? 8 : 8;
+  s.groups = cus < kMaxGroups ? cus : kMaxGroups;
+  s.o = align256((size_t)2 * s.groups * s.rows * head_dim * 4);
+  s.ml = align256((size_t)2 * s.groups * s.rows * 8);
   s.desc = align256((size_t)s.groups * sizeof(Args::Desc));
   return s;
 }
@@ -832,8 +879,13 @@ template <typename T, int D, int S, int RG> int launch(const Args& a, hipStream_
     attr_set.fetch_or(bit, std::memory_order_acq_rel);
   }
   hipLaunchKernelGGL((varlen_kernel<T, D, S, RG>), dim3((unsigned)a.groups), dim3(C::kWaves * 64), C::kLds, s, a);
-  hipLaunchKernelGGL((combine_kernel<T, D, RG>), dim3((unsigned)a.groups, RG), dim3(join_split<RG>() * D * 2), 0, s, a);
+  hipLaunchKernelGGL((combine_kernel<T, D, RG>), dim3((unsigned)a.groups * 4), dim3(256), 0, s, a);
   return hipGetLastError() == hipSuccess ? TSFA_OK : TSFA_ERR_LAUNCH;
+}
+
+template <typename T, int D> int launch_tiles(const Args& a, int rows, hipStream_t s) {
+  if (rows == 32) return launch<T, D, 4, 1>(a, s);
+  return rows == 128 ? launch<T, D, 2, 4>(a, s) : launch<T, D, 1, 8>(a, s);
 }
 
 }  // namespace varlen
@@ -895,8 +947,7 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
   a.mask_n = mask_n;
   a.seqs = make_seqs(q_indptr, kv_lens, kv_indptr, kv_indices, n_indices, page_table_stride, page_table_width, n_pages,
                      page_size, batch, total_q);
-  a.cut = paged::make_cut(sz.few_rows ? 32 : 128, sz.few_rows ? 128 : 64, num_heads / num_kv_heads, num_kv_heads,
-                          mask == nullptr);
+  a.cut = paged::make_cut(sz.rows, 32 * sz.streams, num_heads / num_kv_heads, num_kv_heads, mask == nullptr, sz.extra);
   a.sqn = q_strides[0], a.sqh = q_strides[1];
   a.son = o_strides[0], a.soh = o_strides[1];
   a.cp = cache_strides[0], a.cs = cache_strides[1], a.cr = cache_strides[2], a.ch = cache_strides[3];
@@ -910,10 +961,8 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
   a.ws_ml = reinterpret_cast<float2*>(ws + sz.o);
   a.ws_desc = reinterpret_cast<varlen::Args::Desc*>(ws + sz.o + sz.ml);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == TSFA_DTYPE_BF16) {
-    if (head_dim == 128) return sz.few_rows ? varlen::launch<__bf16, 128, 4, 1>(a, s) : varlen::launch<__bf16, 128, 2, 4>(a, s);
-    return sz.few_rows ? varlen::launch<__bf16, 64, 4, 1>(a, s) : varlen::launch<__bf16, 64, 2, 4>(a, s);
-  }
-  if (head_dim == 128) return sz.few_rows ? varlen::launch<_Float16, 128, 4, 1>(a, s) : varlen::launch<_Float16, 128, 2, 4>(a, s);
-  return sz.few_rows ? varlen::launch<_Float16, 64, 4, 1>(a, s) : varlen::launch<_Float16, 64, 2, 4>(a, s);
+  if (dtype == TSFA_DTYPE_BF16)
+    return head_dim == 128 ? varlen::launch_tiles<__bf16, 128>(a, sz.rows, s) : varlen::launch_tiles<__bf16, 64>(a, sz.rows, s);
+  return head_dim == 128 ? varlen::launch_tiles<_Float16, 128>(a, sz.rows, s)
+                         : varlen::launch_tiles<_Float16, 64>(a, sz.rows, s);
 }

@@ -51,7 +51,7 @@ int main() {
     Seqs s = make_seqs(qi.data(), kl.data(), dense ? nullptr : pi.data(), indices.data(), (int64_t)indices.size(),
                        width, width, 4, 1 << page_shift, batch, total_q);
     const int rg = 1 << pick(0, 3), streams = 1 << pick(0, 2);
-    const Cut c = make_cut(32 * rg, 32 * streams, pick(1, 9), pick(1, 4), pick(0, 1));
+    const Cut c = make_cut(32 * rg, 32 * streams, pick(1, 9), pick(1, 4), pick(0, 1), pick(0, 9));
     const int groups = pick(0, 1) ? 256 : pick(1, 40);
 
     int64_t total = 0;
