@@ -118,6 +118,13 @@ template <int N> __device__ inline void dma_rows(const void* base, const uint32_
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
+// max(a, b, c) in one instruction (fmaxf first quiets operands the compiler
+// cannot prove canonical, one more instruction each).
+__device__ inline float max3f(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 template <int N> __device__ inline void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 // At most `left` units of LPW loads each still on their way (left <= K).
 template <int LPW, int K> __device__ inline void wait_units(int left) {
@@ -196,7 +203,7 @@ template <int D, int S, int RG> struct Shape {
   static constexpr int kLpw = kUnit / 1024 / RG;           // 1 KB loads of a wave per unit
   static constexpr int kRing = S * kStages * kUnit;
   static constexpr int kWords = kTreeUnits * kRows * 4;
-  static constexpr int kLds = kRing + kTableIds * 4 + kWords;
+  static constexpr int kLds = kRing + kTableIds * 8 + kWords;
 };
 
 template <typename T, int D, int S, int RG>
@@ -215,10 +222,11 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   constexpr int GW = LPW < GL ? LPW : GL;  // loads of such a group that a wave makes
   constexpr int NG = LPW / GW;             // groups a wave moves, or shares, per unit
   constexpr bool PIPE = NST >= 4;  // the next unit's scores run under this unit's softmax
+  constexpr int STAG = S == 1 && NST >= 8 ? 1 : 0;  // half of the waves a product behind
   static_assert(NG >= 1 && LPW % GW == 0 && GL % GW == 0 && LPW * (NST - 1) < 64 && NST >= 2, "ring");
   extern __shared__ __attribute__((aligned(256))) unsigned char smem[];
-  int32_t* table = reinterpret_cast<int32_t*>(smem + C::kRing);
-  uint32_t* words = reinterpret_cast<uint32_t*>(smem + C::kRing + kTableIds * 4);
+  int64_t* table = reinterpret_cast<int64_t*>(smem + C::kRing);  // byte offsets of the chunk's pages in the pool
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem + C::kRing + kTableIds * 8);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -284,13 +292,16 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   // (groups of 16 key rows, 0 and 1 K's, 2 and 3 V's).  Chunk x of row k lies
   // at chunk x ^ swz(k), and both swizzles have a period that divides 16.
   const uint32_t ring = lds_addr(smem) + (uint32_t)(st * NST * C::kUnit);
-  uint32_t off_k[GW], off_v[GW];
+  constexpr bool BOTH = RG == 1;  // with more row groups a wave moves K or V
+  const bool moves_v = !BOTH && rg >= RG / 2;
+  uint32_t off[BOTH ? 2 : 1][GW];
 #pragma unroll
   for (int i = 0; i < GW; ++i) {
     const int row = (rg * LPW % GL + i) * RPL + lane / CPR;
     const uint32_t at_row = (uint32_t)row * (uint32_t)a.cr * 2u - (uint32_t)i * 1024u;
-    off_k[i] = at_row + (uint32_t)(((lane % CPR) ^ swz_k<D>(row)) << 4);
-    off_v[i] = at_row + (uint32_t)(((lane % CPR) ^ swz_v<D>(row)) << 4);
+#pragma unroll
+    for (int y = 0; y < (BOTH ? 2 : 1); ++y)
+      off[y][i] = at_row + (uint32_t)(((lane % CPR) ^ ((BOTH ? y == 1 : moves_v) ? swz_v<D>(row) : swz_k<D>(row))) << 4);
   }
 
   for (;;) {
@@ -322,7 +333,9 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     float m_run = -INFINITY, m_lim = -INFINITY, l_run = 0.f;
     const float thr = kRescaleLog2 / sl2;
 
-    const T* hbase = static_cast<const T*>(a.cache) + pl.kvh * a.ch;
+    const char* hbase = reinterpret_cast<const char*>(static_cast<const T*>(a.cache) + pl.kvh * a.ch);
+    const int64_t v_at = a.cs * 2;  // V's bytes behind K's
+    const char* wbase = hbase + (moves_v ? v_at : 0);
     const int kl = sq.kv_len, P = sq.prefix;
     const int mask_cols = a.mask != nullptr ? min(min(sq.q_len, a.mask_n), kl - P) : 0;
     // keys that every row of the tile sees: the prefix, or up to the tile's
@@ -351,35 +364,32 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       const paged::Chunk ck = paged::chunk_of(sq, ps, S, c0, s1, a.mask != nullptr);
       const int c1 = ck.end, first_page = ck.first_page, ids = ck.ids, ut0 = ck.tree_unit;
       for (int i = tid; i < ids; i += C::kWaves * 64)
-        table[i] = min(max(a.seqs.kv_indices[sq.list + first_page + i], 0), a.seqs.n_pages - 1);
+        table[i] = min(max(a.seqs.kv_indices[sq.list + first_page + i], 0), a.seqs.n_pages - 1) * (a.cp * 2);
       barrier();
 
       // Unit j of the chunk's stream into stage j % NST.  Units that reach past
       // the last key take their rows load by load, each from a block that holds
       // a key, so that no stale value of the pool enters P V.
       const int n = c1 - c0;
-      // page ids of the next unit to request, read from the table a step ahead
-      int next_id[NG];
+      // the pages of the next unit to request, read from the table a step ahead
+      int64_t next_page[NG];
       auto peek = [&](int j) {
         const int k0 = ((c0 + j) * S + st) * 32;
 #pragma unroll
         for (int x = 0; x < NG; ++x)
-          next_id[x] = table[min((min(k0 + 16 * ((rg * LPW / GL + x) & 1), kl - 1) >> ps) - first_page, kTableIds - 1)];
+          next_page[x] = table[min((min(k0 + 16 * ((rg * LPW / GL + x) & 1), kl - 1) >> ps) - first_page, kTableIds - 1)];
       };
       peek(0);
       auto issue = [&](int j) {
         const int k0 = ((c0 + j) * S + st) * 32;
-        const uint32_t dst = ring + (uint32_t)((j % NST) * C::kUnit);
+        const uint32_t dst = ring + (uint32_t)j % NST * C::kUnit;
         if (k0 + 32 <= kl) {
 #pragma unroll
           for (int x = 0; x < NG; ++x) {
-            const int grp = rg * LPW / GL + x;
-            const int key = k0 + 16 * (grp & 1);
-            const int id = __builtin_amdgcn_readfirstlane(next_id[x]);
-            const T* base = hbase + id * a.cp + (grp >= 2 ? a.cs : 0) + (int64_t)(key & ((1 << ps) - 1)) * a.cr;
-            const uint32_t to = dst + (uint32_t)(rg * LPW + x * GW) * 1024u;
-            if (grp >= 2) dma_rows<GW>(base, off_v, to);
-            else dma_rows<GW>(base, off_k, to);
+            const uint32_t row = (uint32_t)(k0 + 16 * ((rg * LPW / GL + x) & 1)) & ((1u << ps) - 1u);
+            const bool v_of_both = BOTH && x >= NG / 2;
+            const char* base = wbase + (v_of_both ? v_at : 0) + uniform64(next_page[x]) + (uint64_t)row * ((uint32_t)a.cr * 2u);
+            dma_rows<GW>(base, off[v_of_both ? 1 : 0], dst + (uint32_t)(rg * LPW + x * GW) * 1024u);
           }
         } else {
           for (int x = 0; x < LPW; ++x) {
@@ -387,8 +397,8 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
             const bool is_v = u >= 2 * GL;
             const int kb = (u % (2 * GL)) * RPL;
             const int blk = paged::load_block(k0 + kb, RPL, kl);
-            const int id = __builtin_amdgcn_readfirstlane(table[(blk >> ps) - first_page]);
-            const T* base = hbase + id * a.cp + (is_v ? a.cs : 0) + (int64_t)(blk & ((1 << ps) - 1)) * a.cr;
+            const char* base = hbase + (is_v ? v_at : 0) + uniform64(table[(blk >> ps) - first_page]) +
+                               (int64_t)(blk & ((1 << ps) - 1)) * a.cr * 2;
             const int row = kb + lane / CPR;
             const int from = min(lane / CPR, kl - 1 - blk);
             const int chunk = (lane % CPR) ^ (is_v ? swz_v<D>(row) : swz_k<D>(row));
@@ -427,27 +437,26 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       auto none = [](auto...) {};
       int issued = 0;
 
-      // Unit j, whose scores are in s: online softmax, O^T += V^T P^T.  NEXT: a
-      // unit that every row sees whole, unit j + 1's scores (left in s) between
-      // its exponentials; else the unit may need its mask and stands alone.
-      auto unit = [&](auto next_c, int j, f32x16& s) {
+      // Unit j, whose scores are in s: its row statistics and P (rounded pairs
+      // in pk), O re-based where needed.  NEXT: a unit that every row sees
+      // whole, unit j + 1's scores (left in s) between its exponentials; else
+      // the unit may need its mask (w: the row's visible keys).
+      auto soft = [&](auto next_c, int j, f32x16& s, uint32_t (&pk)[8], uint32_t& w) {
         constexpr bool NEXT = decltype(next_c)::value;
-        const unsigned char* vt = smem + (st * NST + j % NST) * C::kUnit + C::kTile;
         const int u = (c0 + j) * S + st;
-        const bool masked = !NEXT && (u + 1) * 32 > seen_by_all;
-        uint32_t w = 0xffffffffu;
         float alpha, ms;
         bool need;
         auto stats = [&]() {
-          if (masked) {
+          if (!NEXT && (u + 1) * 32 > seen_by_all) {
             w = a.mask != nullptr ? words[(u - ut0) * M + rg * 32 + ln] : word_of(u * 32, t);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (!((w >> (8 * (i >> 2) + 4 * lh + (i & 3))) & 1u)) s[i] = -INFINITY;
           }
-          float mx = s[0];
+          float mx = max3f(s[0], s[1], s[2]);
 #pragma unroll
-          for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+          for (int i = 3; i < 15; i += 2) mx = max3f(mx, s[i], s[i + 1]);
+          mx = max3f(mx, s[15], s[15]);
           const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
           const float rmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
           // the reference point moves only when a score passes it by more than
@@ -463,7 +472,6 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         // 16-bit operands; its row sum takes the unrounded values.  Pinned where
         // they are computed: the compiler sinks them past the re-base otherwise.
         float psum = 0.f, p[16];
-        uint32_t pk[8];
         auto expo = [&](int i) {
           p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl2, -ms));
           psum += p[i];
@@ -473,7 +481,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           }
         };
         if constexpr (NEXT) {
-          const f32x16 sn = scores(smem + (st * NST + (j + 1) % NST) * C::kUnit, [&]() {
+          const f32x16 sn = scores(smem + (st * NST + (uint32_t)(j + 1) % NST) * C::kUnit, [&]() {
             if (issued < n) issue(issued++);
             stats();
           }, [&](int kk) {
@@ -491,26 +499,28 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
         }
+      };
 
-        // V^T by the transposing LDS read: lane i of 16-lane group x gets keys
-        // 16 s2 + 8 jj + 4 (x >> 1) + [0, 4) of d = 32 dt + 16 (x & 1) + i, the
-        // key order in which P lies
+      // O^T += V^T P^T of unit j.  V^T by the transposing LDS read: lane i of
+      // 16-lane group x gets keys 16 s2 + 8 jj + 4 (x >> 1) + [0, 4) of
+      // d = 32 dt + 16 (x & 1) + i, the key order in which P lies; products of
+      // one d tile lie DT apart.
+      auto pv = [&](auto next_c, int j, const uint32_t (&pk)[8], uint32_t w) {
+        constexpr bool NEXT = decltype(next_c)::value;
+        const unsigned char* vt = smem + (st * NST + (uint32_t)j % NST) * C::kUnit + C::kTile;
         const V8 pb[2] = {bit_cast<V8>(U4{pk[0], pk[1], pk[2], pk[3]}), bit_cast<V8>(U4{pk[4], pk[5], pk[6], pk[7]})};
         const int vx = lane >> 4, vi = lane & 15;
         const int vrow = 4 * (vx >> 1) + (vi >> 2);
         const int vch = 2 * (vx & 1) + ((vi & 3) >> 1), vhalf = 8 * (vi & 1);
-        const uint32_t vb = lds_addr(vt) + (uint32_t)(vrow * C::kRowBytes + vhalf);
+        const uint32_t vb = lds_addr(vt) + (uint32_t)(vrow * C::kRowBytes + ((vch ^ swz_v<D>(vrow)) << 4) + vhalf);
         i16x4 vh[2 * DT][2];
-        auto rv = [&](int x) {
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj)
-            vh[x][jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (TSFA_LDS i16x4*)(uintptr_t)(vb + (uint32_t)((16 * (x & 1) + 8 * jj) * C::kRowBytes +
-                                                             (((4 * (x >> 1) + vch) ^ swz_v<D>(vrow)) << 4))));
+        auto rv = [&](int x) {  // x = s2 DT + dt: dt moves offset bits 6 and 7 under the XOR
+          const TSFA_LDS char* at = (const TSFA_LDS char*)(uintptr_t)(vb ^ (uint32_t)((x % DT) << 6));
+          vh[x][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TSFA_LDS i16x4*)(at + 16 * (x / DT) * C::kRowBytes));
+          vh[x][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TSFA_LDS i16x4*)(at + (16 * (x / DT) + 8) * C::kRowBytes));
         };
-        auto vf = [&](int x) { return __builtin_shufflevector(vh[x][0], vh[x][1], 0, 1, 2, 3, 4, 5, 6, 7); };
         bool odd = false;
-        if (masked) {
+        if (!NEXT && ((c0 + j) * S + st + 1) * 32 > seen_by_all) {
           // infinities and NaN of keys that some rows do not see: 0 * NaN must
           // not reach those rows, so they leave the product and are added to
           // the rows that see them
@@ -529,13 +539,13 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
 #pragma unroll
         for (int x = 0; x < 2 * DT; ++x) {
           if (x + VA < 2 * DT) rv(x + VA);
-          i16x8 f = vf(x);
+          i16x8 f = __builtin_shufflevector(vh[x][0], vh[x][1], 0, 1, 2, 3, 4, 5, 6, 7);
           if (!NEXT && odd) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               if ((f[e] & (short)(EXP2 & 0xffff)) == (short)(EXP2 & 0xffff)) f[e] = 0;
           }
-          o[x >> 1] = Mma<T>::run(bit_cast<V8>(f), pb[x & 1], o[x >> 1]);
+          o[x % DT] = Mma<T>::run(bit_cast<V8>(f), pb[x / DT], o[x % DT]);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (!NEXT && odd) {
@@ -557,7 +567,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       };
 
       vm_wait<0>();  // the ring's waits count its own loads alone
-      while (issued < NST - 1 && issued < n) issue(issued++);
+      while (issued < NST - 1 - STAG && issued < n) issue(issued++);
       if (a.mask != nullptr) {
         // under the first units' way here; the barriers below order them
         for (int i = tid; i < (c1 * S - ut0) * M; i += C::kWaves * 64) {
@@ -569,23 +579,39 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       wait_units<LPW, NST - 2>(issued - 1);
       barrier();
       f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
+      uint32_t pk[8], w = 0xffffffffu;
+      constexpr std::true_type full{};
+      constexpr std::false_type part{};
       if constexpr (PIPE) {
-        // steps whose units every row of the tile sees whole
+        // Steps whose units every row of the tile sees whole.  Past barrier j
+        // unit j + 1 is there, and every wave is done with unit j - 1 (with
+        // STAG, j - 2).  With STAG half of the waves meet at barrier j + 1
+        // before the product of unit j: the other wave of their SIMD is then at
+        // its exponentials while they run it, and the other way round.
         const int n_full = min(n, seen_by_all / (32 * S) - c0);
-        for (; j + 1 < n_full; ++j) {
-          // unit j + 1 is there, and every wave is done with unit j - 1
-          wait_units<LPW, NST - 3>(issued - 2 - j);
+        const bool late = STAG != 0 && rg >= RG / 2;
+        auto meet = [&](int i) {
+          if (issued < n) vm_wait<(NST - 3 - STAG) * LPW>();
+          else wait_units<LPW, NST - 3>(issued - 2 - i);
           barrier();
-          unit(std::true_type{}, j, s);
+        };
+        if (late && n_full > 1) meet(0);
+        for (; j + 1 < n_full; ++j) {
+          if (!late) meet(j);
+          soft(full, j, s, pk, w);
+          if (late && j + 2 < n_full) meet(j + 1);
+          pv(full, j, pk, w);
         }
       }
       for (;;) {
-        unit(std::false_type{}, j, s);
+        w = 0xffffffffu;
+        soft(part, j, s, pk, w);
+        pv(part, j, pk, w);
         if (++j >= n) break;
         wait_units<LPW, NST - 2>(issued - 1 - j);
         barrier();  // unit j is there, and every wave is done with unit j - 1
         while (issued < min(n, j + NST)) issue(issued++);
-        s = scores(smem + (st * NST + j % NST) * C::kUnit, none, none);
+        s = scores(smem + (st * NST + (uint32_t)j % NST) * C::kUnit, none, none);
       }
       barrier();  // the rings, the table and the words are free again
       c0 = c1;
@@ -598,7 +624,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     constexpr int X = D / 8, XS = X / S;
     const bool whole = s0 == 0 && s1 == n_steps;
     float4* jo = reinterpret_cast<float4*>(smem);                              // the streams' O
-    float2* jml = reinterpret_cast<float2*>(smem + C::kRing + kTableIds * 4);  // [S][RG][32] (m, l)
+    float2* jml = reinterpret_cast<float2*>(smem + C::kRing + kTableIds * 8);  // [S][RG][32] (m, l)
     static_assert(S * RG * 32 * 8 <= C::kWords && (S == 1 || S * RG * X * 1024 <= C::kRing), "join");
     if (S > 1 && lh == 0) jml[(st * RG + rg) * 32 + ln] = make_float2(m_run, l_run);
     float mm = -INFINITY, ll = 0.f, fs[S];
@@ -709,13 +735,62 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
 }
 
 // Joins the parts of the tiles that several runs share.  Work items are (tile,
-// row group, d tile): every block lists the tiles first (one load of all runs'
-// descriptors) and takes items blockIdx.x, + gridDim.x, ...; its four waves
-// split the parts, kJoin of them loaded at once.  A block per run would leave
-// most of them empty and the others few: 17 us against %JOIN% us for 16 tiles
-// in 14 parts each.
+// row group, d tile); every block lists the tiles first (one load of all runs'
+// descriptors).  Tiles of up to kJoin parts take a wave per item, longer ones a
+// block whose four waves split the parts, kJoin of them loaded at once.  (A
+// block per run would leave most of them empty and the others few: 17 us against
+// 6 for 16 tiles in 14 parts each.)
 constexpr int kJoin = 4;
 constexpr int kMaxGroups = 1024;
+
+// Parts p0, p0 + step, ... of a lane's row and d tile, joined into (m, l, o).
+template <int D, int RG>
+__device__ inline void join_parts(const Args& a, const Args::Desc& desc, int run, int rg, int dt, int p0, int step,
+                                  int lane, float& m, float& l, float4 (&o)[4]) {
+  constexpr int M = 32 * RG;
+  const float sl2 = a.scale_log2;
+  for (; p0 < desc.runs; p0 += step * kJoin) {
+    float2 x[kJoin];
+    float4 v[kJoin][4];
+    bool has[kJoin];
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      // past the last and runs without a step of the tile: loaded, not used
+      const int p = min(p0 + step * k, desc.runs - 1);
+      has[k] = p0 + step * k < desc.runs &&
+               paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
+      const int64_t slot = p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p);
+      x[k] = a.ws_ml[slot * M + rg * 32 + (lane & 31)];
+      const float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8) + 4 * dt) * 64 + lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[k][i] = wo[i * 64];
+      if (!has[k]) x[k] = make_float2(-INFINITY, 0.f);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) m_new = fmaxf(m_new, x[k].x);
+    const float m0 = m_new == -INFINITY ? 0.f : m_new;
+    const float fa = __builtin_amdgcn_exp2f((m - m0) * sl2);
+    m = m_new;
+    l *= fa;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(o[i].x * fa, o[i].y * fa, o[i].z * fa, o[i].w * fa);
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      if (!has[k]) continue;
+      const float f = __builtin_amdgcn_exp2f((x[k].x - m0) * sl2);
+      l += x[k].y * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i].x += v[k][i].x * f;
+        o[i].y += v[k][i].y * f;
+        o[i].z += v[k][i].z * f;
+        o[i].w += v[k][i].w * f;
+      }
+    }
+  }
+}
+
 template <typename T, int D, int RG>
 __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   typedef T T4 __attribute__((ext_vector_type(4)));
@@ -724,12 +799,16 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   __shared__ float2 jml[PS * 64];
   __shared__ short tiles[kMaxGroups];
   __shared__ int wave_count[kMaxGroups / 64];
+  __shared__ int any_long;
   const int lane = threadIdx.x & 63, ps = threadIdx.x >> 6;
   const int ln = lane & 31, lh = lane >> 5;
+  if (threadIdx.x == 0) any_long = 0;
+  __syncthreads();
   for (int r0 = ps * 64; r0 < a.groups; r0 += 256) {
-    const bool on = r0 + lane < a.groups && a.ws_desc[r0 + lane].runs != 0;
-    const uint64_t set = __ballot(on);
+    const int runs = r0 + lane < a.groups ? a.ws_desc[r0 + lane].runs : 0;
+    const uint64_t set = __ballot(runs != 0);
     if (lane == 0) wave_count[r0 / 64] = __builtin_popcountll(set);
+    if (runs > kJoin) any_long = 1;
   }
   __syncthreads();
   int n_tiles = 0;
@@ -745,56 +824,40 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   }
   __syncthreads();
   const float sl2 = a.scale_log2;
+  // float4 x of the lane's row and d tile: normalised, rounded and written
+  auto put = [&](const Args::Desc& desc, const Seq& sq, int rg, int dt, int x, float4 r, float m, float l) {
+    const int G = a.cut.group, row = desc.tile * M + rg * 32 + ln;
+    if (row >= sq.q_len * G) return;
+    const int t = (int)fdiv((uint32_t)row, a.cut.by_group), h = desc.kvh * G + (row - t * G);
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const T4 v = {(T)(r.x * inv), (T)(r.y * inv), (T)(r.z * inv), (T)(r.w * inv)};
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt +
+                           8 * x + 4 * lh) = v;
+    if (a.lse != nullptr && dt == 0 && x == 0 && lh == 0)
+      a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] = l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
+  };
+  for (int item = blockIdx.x * PS + ps; item < n_items; item += gridDim.x * PS) {
+    const int run = tiles[item / (RG * DT)], rg = item / DT % RG, dt = item % DT;
+    const Args::Desc desc = a.ws_desc[run];
+    if (desc.runs > kJoin) continue;
+    const Seq sq = paged::seq_of(a.seqs, desc.b);
+    if (desc.tile * M + rg * 32 >= sq.q_len * a.cut.group) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 o[4] = {};
+    join_parts<D, RG>(a, desc, run, rg, dt, 0, 1, lane, m, l, o);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) put(desc, sq, rg, dt, x, o[x], m, l);
+  }
+  if (any_long == 0) return;
   for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
     const int run = tiles[item / (RG * DT)], rg = item / DT % RG, dt = item % DT;
     const Args::Desc desc = a.ws_desc[run];
-    const int parts = desc.runs;
+    if (desc.runs <= kJoin) continue;
     const Seq sq = paged::seq_of(a.seqs, desc.b);
-    const int G = a.cut.group, TG = sq.q_len * G;
-    if (desc.tile * M + rg * 32 >= TG) continue;
+    if (desc.tile * M + rg * 32 >= sq.q_len * a.cut.group) continue;
     float m = -INFINITY, l = 0.f;
-    float4 o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = ps; p0 < parts; p0 += PS * kJoin) {
-      float2 x[kJoin];
-      float4 v[kJoin][4];
-      bool has[kJoin];
-#pragma unroll
-      for (int k = 0; k < kJoin; ++k) {
-        // past the last and runs without a step of the tile: loaded, not used
-        const int p = min(p0 + PS * k, parts - 1);
-        has[k] = p0 + PS * k < parts && paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
-        const int64_t slot = p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p);
-        x[k] = a.ws_ml[slot * M + rg * 32 + ln];
-        const float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8) + 4 * dt) * 64 + lane;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[k][i] = wo[i * 64];
-        if (!has[k]) x[k] = make_float2(-INFINITY, 0.f);
-      }
-      float m_new = m;
-#pragma unroll
-      for (int k = 0; k < kJoin; ++k) m_new = fmaxf(m_new, x[k].x);
-      const float m0 = m_new == -INFINITY ? 0.f : m_new;
-      const float fa = __builtin_amdgcn_exp2f((m - m0) * sl2);
-      m = m_new;
-      l *= fa;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = make_float4(o[i].x * fa, o[i].y * fa, o[i].z * fa, o[i].w * fa);
-#pragma unroll
-      for (int k = 0; k < kJoin; ++k) {
-        if (!has[k]) continue;
-        const float f = __builtin_amdgcn_exp2f((x[k].x - m0) * sl2);
-        l += x[k].y * f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[i].x += v[k][i].x * f;
-          o[i].y += v[k][i].y * f;
-          o[i].z += v[k][i].z * f;
-          o[i].w += v[k][i].w * f;
-        }
-      }
-    }
+    float4 o[4] = {};
+    join_parts<D, RG>(a, desc, run, rg, dt, ps, PS, lane, m, l, o);
     jml[ps * 64 + lane] = make_float2(m, l);
 #pragma unroll
     for (int i = 0; i < 4; ++i) jo[(ps * 4 + i) * 64 + lane] = o[i];
@@ -817,17 +880,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
       r.z += v.z * f;
       r.w += v.w * f;
     }
-    const int row = desc.tile * M + rg * 32 + ln;
-    if (row < TG) {
-      const int t = (int)fdiv((uint32_t)row, a.cut.by_group), h = desc.kvh * G + (row - t * G);
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const T4 v = {(T)(r.x * inv), (T)(r.y * inv), (T)(r.z * inv), (T)(r.w * inv)};
-      *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt +
-                             8 * ps + 4 * lh) = v;
-      if (a.lse != nullptr && dt == 0 && ps == 0 && lh == 0)
-        a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] =
-            l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
-    }
+    put(desc, sq, rg, dt, ps, r, m, l);
     __syncthreads();  // jo and jml are written again
   }
 }
