@@ -16,6 +16,7 @@
 //   states_kernel the states' rows of the selected parents.
 #include <hip/hip_runtime.h>
 
+#include <float.h>
 #include <math.h>
 
 #include "tsfa_internal.h"
@@ -27,6 +28,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxK = 64;
 constexpr int kMaxBeams = 256;
 constexpr int kMaxStates = 8;
+constexpr int kFullCard = 512;  // workgroups
 constexpr int64_t kStatesInside = 256 << 10;
 
 // Statistics of one tile: maximum (as a float) and sum of exp(x - maximum).
@@ -44,14 +46,18 @@ struct PartArgs {
   PartStat* stats;  // [rows][tiles]
 };
 
-// A candidate of a row as one number, better = larger: the logit in an order
-// of its bits that integers compare alike (-0 counts as 0), then the lower
-// token.  0 is no candidate (-inf, NaN, past the row).
-__device__ inline uint64_t make_key(float x, uint32_t v) {
+// A logit in an order of its bits that integers compare alike (-0 counts as
+// 0); 0 is no candidate (-inf, NaN).
+__device__ inline uint32_t order_of(float x) {
   if (!(x > -INFINITY)) return 0;
   const uint32_t u = __float_as_uint(x + 0.0f);
-  const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
-  return ((uint64_t)o << 32) | (uint32_t)~v;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+// A candidate of a row as one number, better = larger: its order, then the
+// lower token.
+__device__ inline uint64_t make_key(float x, uint32_t v) {
+  const uint32_t o = order_of(x);
+  return o == 0 ? 0 : ((uint64_t)o << 32) | (uint32_t)~v;
 }
 __device__ inline float key_logit(uint64_t key) {
   const uint32_t o = (uint32_t)(key >> 32);
@@ -59,62 +65,63 @@ __device__ inline float key_logit(uint64_t key) {
 }
 __device__ inline uint32_t key_token(uint64_t key) { return ~(uint32_t)key; }
 
-// 2^(x log2 e) for x <= 0 (below -700: the value at -700, which no sum of
-// such weights notices): x log2 e = n + f, 2^f by the polynomial of degree 9
-// through the Chebyshev points of [-1/2, 1/2] (2e-14 off at most), n into the
+// 2^t for -1000 < t <= 0: t = n + f, 2^f by the polynomial of degree 8 through
+// the Chebyshev points of [-1/2, 1/2] (1.1e-12 off at most), n into the
 // exponent.  Adding 1.5 * 2^52 rounds to n and leaves it in the low word.
-__device__ inline double exp_neg(double x) {
+__device__ inline double exp2_neg(double t) {
   constexpr double kRound = 6755399441055744.0;
-  const double t = fmax(x, -700.0) * 1.4426950408889634074;
   const double u = t + kRound;
   const double f = t - (u - kRound);
-  double p = 1.0205905413765595e-07;
-  p = fma(p, f, 1.325964524488711e-06);
-  p = fma(p, f, 1.5252672924850737e-05);
-  p = fma(p, f, 0.0001540343375125101);
-  p = fma(p, f, 0.0013333558200794592);
-  p = fma(p, f, 0.009618129193934313);
-  p = fma(p, f, 0.05550410866465167);
-  p = fma(p, f, 0.2402265069564034);
-  p = fma(p, f, 0.6931471805599462);
-  p = fma(p, f, 1.0000000000000135);
+  double p = 1.3255224878668817e-06;
+  p = fma(p, f, 1.5310079402249296e-05);
+  p = fma(p, f, 0.00015403455852453838);
+  p = fma(p, f, 0.0013333450568000645);
+  p = fma(p, f, 0.009618129159402558);
+  p = fma(p, f, 0.05550410941205933);
+  p = fma(p, f, 0.2402265069581299);
+  p = fma(p, f, 0.6931471805459335);
+  p = fma(p, f, 1.0);
   const uint64_t bits = __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, u) << 52);
   return __builtin_bit_cast(double, bits);
 }
-// exp(x - top) for x <= top, top > -inf; equal infinities weigh 1.
-__device__ inline double weight(float x, float top) { return x == top ? 1.0 : exp_neg((double)x - (double)top); }
+constexpr double kLog2e = 1.4426950408889634074;
+// exp(x - top) for x <= top, top > -inf; equal infinities weigh 1 (below -600:
+// the weight at -600, which no sum notices).
+__device__ inline double weight(float x, float top) {
+  if (x == top) return 1.0;
+  return exp2_neg(fmax((double)x - (double)top, -600.0) * kLog2e);
+}
 
-// The largest v that at least k of the wave's keys a and b are not below, from
-// the top bit down by counting lanes; 1 if fewer than k are not 0.  Keys of
-// distinct candidates differ, so exactly k keys reach it.
-__device__ inline uint64_t kth_key(uint64_t a, uint64_t b, int k) {
-  auto count = [](bool x, bool y) { return __builtin_popcountll(__ballot(x)) + __builtin_popcountll(__ballot(y)); };
-  if (count(a != 0, b != 0) < k) return 1;
-  const uint32_t ah = (uint32_t)(a >> 32), bh = (uint32_t)(b >> 32);
-  uint32_t hi = 0;
+// A bound that at least k of the wave's values reach (0: no value, never
+// counted), and not many more unless they tie; 1 if fewer than k are there.
+// From the top bit down by counting lanes, N values to a lane.
+template <int N> __device__ inline uint32_t kth_order(const uint32_t (&x)[N], int k) {
+  auto count = [&](uint32_t bound) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) c += __builtin_popcountll(__ballot(x[i] >= bound));
+    return c;
+  };
+  if (count(1) < k) return 1;
+  uint32_t v = 0;
   for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
-    const int c = count(ah >= (hi | bit), bh >= (hi | bit));
-    if (c >= k) hi |= bit;
-    if (c == k) return (uint64_t)hi << 32;
+    const int c = count(v | bit);
+    if (c < k) continue;
+    v |= bit;
+    if (c <= k + k / 2 + 4) break;
   }
-  const int above = count(ah > hi, bh > hi);
-  uint32_t lo = 0;
-  for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
-    const int c = above + count(ah == hi && (uint32_t)a >= (lo | bit), bh == hi && (uint32_t)b >= (lo | bit));
-    if (c >= k) lo |= bit;
-    if (c == k) break;
-  }
-  return ((uint64_t)hi << 32) | lo;
+  return v;
 }
 
 // EPT elements per thread, VEC of them in one 16-byte load.
 template <typename T, int EPT>
 __global__ __launch_bounds__(kThreads) void part_kernel(const PartArgs a) {
-  constexpr int VEC = 16 / (int)sizeof(T), NU = EPT / VEC, NW = kThreads / 64, H = EPT / 2;
-  __shared__ __attribute__((aligned(16))) uint64_t list[2 * kMaxK * EPT];
+  constexpr int VEC = 16 / (int)sizeof(T), NU = EPT / VEC, NW = kThreads / 64;
+  extern __shared__ __attribute__((aligned(16))) uint64_t list[];  // k * EPT
+  __shared__ uint32_t orders[kThreads];
   __shared__ double wsum[NW];
   __shared__ float wtop[NW];
-  __shared__ uint64_t wbound[NW];
+  __shared__ uint32_t bound;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tile = blockIdx.x % a.tiles, row = blockIdx.x / a.tiles;
@@ -139,66 +146,100 @@ __global__ __launch_bounds__(kThreads) void part_kernel(const PartArgs a) {
   auto token = [&](int e) { return (uint32_t)(v0 + ((e / VEC) * kThreads + tid) * VEC + e % VEC); };
   if (tid == 0) count = 0;
 
-  // the best of each half of the thread's elements (the lowest token of equal
-  // ones: tokens rise with e)
-  float fa = -INFINITY, fb = -INFINITY;
+  float mine = -INFINITY;  // fmaxf passes over NaN, which is no candidate and weighs nothing
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) {
-    if (!(xs[e] == xs[e])) xs[e] = -INFINITY;  // NaN is no candidate and weighs nothing
-    if (e < H) fa = fmaxf(fa, xs[e]);
-    else fb = fmaxf(fb, xs[e]);
-  }
-  int ea = 0, eb = H;
-#pragma unroll
-  for (int e = H - 1; e >= 0; --e) {
-    if (xs[e] == fa) ea = e;
-    if (xs[e + H] == fb) eb = e + H;
-  }
-  const uint64_t ka = make_key(fa, token(ea)), kb = make_key(fb, token(eb));
-  float top = fmaxf(fa, fb);
+  for (int e = 0; e < EPT; ++e) mine = fmaxf(mine, xs[e]);
+  orders[tid] = order_of(mine);
+  float top = mine;
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
-  // Each wave's k-th best half bounds the tile's k-th best element from below,
-  // the best of these bounds closest; at most k halves of every wave reach it,
-  // 2 k EPT elements whatever the values are (a few times k for a model's).
-  const uint64_t wb = kth_key(ka, kb, a.k);
-  if (lane == 0) {
-    wtop[wave] = top;
-    wbound[wave] = wb;
-  }
+  if (lane == 0) wtop[wave] = top;
   __syncthreads();
-  uint64_t lim = 1;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    top = fmaxf(top, wtop[i]);
-    lim = wbound[i] > lim ? wbound[i] : lim;
-  }
-  if (ka >= lim || kb >= lim) {
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      const uint64_t key = make_key(xs[e], token(e));
-      if (key >= lim) list[atomicAdd(&count, 1)] = key;
-    }
-  }
+  for (int i = 0; i < NW; ++i) top = fmaxf(top, wtop[i]);
 
-  double sum = 0, sum2 = 0;
-  if (top == INFINITY) {
+  // The k-th best of the threads' best elements bounds the tile's k-th best
+  // from below: few more than k elements reach it, unless many tie.
+  if (wave == 0) {
+    uint32_t o[NW];
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) sum += xs[e] == top ? 1.0 : 0.0;
-  } else if (top > -INFINITY) {
-    const double t = top;
+    for (int i = 0; i < NW; ++i) o[i] = orders[i * 64 + lane];
+    const uint32_t v = kth_order(o, a.k);
+    if (lane == 0) bound = v;
+  }
+  double sum = 0;
+  if (fabsf(top) <= 4096.0f) {
+    // log2 e x and log2 e top round apart: 4096 * 2^-52 at most
+    const double shift = -(double)top * kLog2e;
+    const float low = top - 88.0f;  // less, NaN and -inf: e^-88, which no sum notices
+    double sum2 = 0;
 #pragma unroll
     for (int e = 0; e < EPT; e += 2) {
-      sum += exp_neg((double)xs[e] - t);
-      sum2 += exp_neg((double)xs[e + 1] - t);
+      sum += exp2_neg(fma((double)fmaxf(xs[e], low), kLog2e, shift));
+      sum2 += exp2_neg(fma((double)fmaxf(xs[e + 1], low), kLog2e, shift));
     }
     sum += sum2;
+  } else if (top > -INFINITY) {
+    // read again: kept for this loop too, they cost the kernel registers, and waves
+#pragma unroll 1
+    for (int e = 0; e < EPT; ++e) {
+      const uint32_t v = token(e);
+      const float y = v < (uint32_t)a.vocab ? (float)x[v] : -INFINITY;
+      if (y > -INFINITY) sum += weight(y, top);
+    }
   }
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
   if (lane == 0) wsum[wave] = sum;
   __syncthreads();
-  const int n = count;
+
+  const int room = a.k * EPT;
+  // the bound as a logit (below every number's order: the least number)
+  const float lim = bound < 0x00800000u ? -FLT_MAX : key_logit((uint64_t)bound << 32);
+  if (mine >= lim) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e)
+      if (xs[e] >= lim) {
+        const int at = atomicAdd(&count, 1);
+        if (at < room) list[at] = make_key(xs[e], token(e));
+      }
+  }
+  __syncthreads();
+  int n = count;
+  if (n > room) {
+    // More ties at the bound than the list holds: the k-th best thread by its
+    // best element's value and token, which only k threads reach, is the bound.
+    auto key_of = [&](int e) {
+      const uint32_t v = token(e);
+      return v < (uint32_t)a.vocab ? make_key((float)x[v], v) : 0;
+    };
+    uint64_t best = 0;
+#pragma unroll 1
+    for (int e = 0; e < EPT; ++e) {
+      const uint64_t key = key_of(e);
+      best = key > best ? key : best;
+    }
+    __shared__ uint64_t bests[kThreads];
+    __shared__ uint64_t exact;
+    bests[tid] = best;
+    if (tid == 0) {
+      count = 0;
+      exact = 1;
+    }
+    __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < kThreads; ++i) rank += bests[i] > best;
+    if (best != 0 && rank == a.k - 1) exact = best;
+    __syncthreads();
+    const uint64_t by = exact;
+#pragma unroll 1
+    for (int e = 0; e < EPT; ++e) {
+      const uint64_t key = key_of(e);
+      if (key >= by) list[atomicAdd(&count, 1)] = key;
+    }
+    __syncthreads();
+    n = count;
+  }
   uint64_t* out = a.keys + ((int64_t)row * a.tiles + tile) * a.k;
   for (int i = tid; i < n; i += kThreads) {
     const uint64_t key = list[i];
@@ -232,8 +273,17 @@ __device__ inline void copy_row(const States& st, int s, int64_t from, int64_t t
   const char* src = static_cast<const char*>(st.src[s]) + from * bytes;
   char* dst = static_cast<char*>(st.dst[s]) + to * bytes;
   if (((reinterpret_cast<uintptr_t>(st.src[s]) | reinterpret_cast<uintptr_t>(st.dst[s]) | (uintptr_t)bytes) & 15) == 0) {
-    for (int64_t i = first; i < bytes / 16; i += step)
-      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    const uint4* s16 = reinterpret_cast<const uint4*>(src);
+    uint4* d16 = reinterpret_cast<uint4*>(dst);
+    int64_t i = first;
+    for (; i + 3 * step < bytes / 16; i += 4 * step) {
+      const uint4 v0 = s16[i], v1 = s16[i + step], v2 = s16[i + 2 * step], v3 = s16[i + 3 * step];
+      d16[i] = v0;
+      d16[i + step] = v1;
+      d16[i + 2 * step] = v2;
+      d16[i + 3 * step] = v3;
+    }
+    for (; i < bytes / 16; i += step) d16[i] = s16[i];
   } else {
     for (int64_t i = first; i < bytes; i += step) dst[i] = src[i];
   }
@@ -281,18 +331,34 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
   __shared__ Cand heads[kMergeThreads];
   __shared__ Cand list[kMergeList];
   __shared__ Cand kept[kMaxK];
-  __shared__ uint64_t wbound[NW];
+  __shared__ uint32_t wbound[NW];
   __shared__ Cand bound;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x;
   const Cand none = {0, 0xffffffffu, 0};
 
+  // candidate c: place p of list l; the round's keys are requested ahead
+  const int lists = a.beams * a.tiles;
+  const int total = lists * a.k;
+  const uint64_t* keys = a.keys + (int64_t)b * total;
+  uint64_t raw[kBatch];
+  auto request = [&](int c0) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const uint32_t c = (uint32_t)(c0 + j * kMergeThreads + tid);
+      const uint32_t p = c / (uint32_t)lists, l = c - p * (uint32_t)lists;
+      raw[j] = c < (uint32_t)total ? keys[(int64_t)l * a.k + p] : 0;
+    }
+  };
+  request(0);
+
   // lse_w = top + log(sum) of the tiles, 16 lanes to a beam; a beam with
   // nothing above -inf, or whose score is not finite, has no candidates
   for (int w0 = 0; w0 < a.beams; w0 += kMergeThreads / 16) {
     const int w = w0 + tid / 16, l = tid & 15;
     const PartStat* st = a.stats + ((int64_t)b * a.beams + (w < a.beams ? w : a.beams - 1)) * a.tiles;
+    const float c = a.scores[b * a.ssb + (w < a.beams ? w : 0) * a.ssw];
     float top = -INFINITY;
     for (int i = l; i < a.tiles; i += 16) top = fmaxf(top, st[i].top);
 #pragma unroll
@@ -303,7 +369,6 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
 #pragma unroll
     for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
     if (l == 0 && w < a.beams) {
-      const float c = a.scores[b * a.ssb + w * a.ssw];
       const bool alive = top > -INFINITY && c - c == 0.0f;
       tops[w] = top;
       score[w] = alive ? (double)c : -INFINITY;
@@ -317,41 +382,39 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
 
   // Candidates in rounds, the tiles' best first, so that the first rounds
   // bring the bound near its end and the later ones find little above it.
-  const int lists = a.beams * a.tiles;
-  const int64_t total = (int64_t)lists * a.k;
-  const uint64_t* keys = a.keys + (int64_t)b * lists * a.k;
-  for (int64_t c0 = 0; c0 < total; c0 += kMergeThreads * kBatch) {
+  for (int c0 = 0; c0 < total; c0 += kMergeThreads * kBatch) {
     const Cand last = kept[a.k - 1];
     Cand cs[kBatch], top = none;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int64_t c = c0 + j * kMergeThreads + tid;
       cs[j] = none;
-      if (c < total) {
-        const int p = (int)((uint32_t)c / (uint32_t)lists), l = (int)((uint32_t)c - (uint32_t)p * (uint32_t)lists);
-        const uint64_t key = keys[(int64_t)l * a.k + p];
-        const int w = l / a.tiles;
-        if (key != 0 && score[w] > -INFINITY) {
-          const float x = key_logit(key);
-          const bool inf = tops[w] == INFINITY;
-          if (!inf || x == INFINITY) {
-            cs[j].value = value_key((score[w] + (inf ? 0.0 : (double)x)) - lse[w]);
-            cs[j].flat = (uint32_t)w * (uint32_t)a.vocab + key_token(key);
-          }
+      if (raw[j] != 0) {
+        const uint32_t c = (uint32_t)(c0 + j * kMergeThreads + tid);
+        const int w = (int)(c % (uint32_t)lists) / a.tiles;
+        const float x = key_logit(raw[j]);
+        const bool inf = tops[w] == INFINITY;
+        if (score[w] > -INFINITY && (!inf || x == INFINITY)) {
+          cs[j].value = value_key((score[w] + (inf ? 0.0 : (double)x)) - lse[w]);
+          cs[j].flat = (uint32_t)w * (uint32_t)a.vocab + key_token(raw[j]);
         }
       }
       if (!better(cs[j], last)) cs[j] = none;
       if (better(cs[j], top)) top = cs[j];
     }
     if (tid == 0) count = 0;
+    if (c0 + kMergeThreads * kBatch < total) request(c0 + kMergeThreads * kBatch);
     if (__syncthreads_or(top.value != 0) == 0) continue;
-    // as in part_kernel, by value alone: ties at the bound stay in
-    const uint64_t wb = kth_key(top.value, 0, a.k);
+    // as in part_kernel, by the upper half of the value: ties stay in
+    const uint32_t hi[1] = {(uint32_t)(top.value >> 32)};
+    const uint32_t wb = kth_order(hi, a.k);
     if (lane == 0) wbound[wave] = wb;
     __syncthreads();
     uint64_t lim = last.value > 1 ? last.value : 1;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) lim = wbound[i] > lim ? wbound[i] : lim;
+    for (int i = 0; i < NW; ++i) {
+      const uint64_t v = wbound[i] > 1 ? (uint64_t)wbound[i] << 32 : 1;
+      lim = v > lim ? v : lim;
+    }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
       if (cs[j].value >= lim) {
@@ -419,11 +482,12 @@ __global__ __launch_bounds__(kThreads) void states_kernel(const States st, const
            (int64_t)gridDim.x * kThreads);
 }
 
-// Elements of a tile per thread: long tiles where the rows alone fill the
-// card, short ones where a row has to be spread over it.
+// Elements of a tile per thread: long tiles where they fill the card, short
+// ones where a row has to be spread over it.
 inline int elements_per_thread(int64_t rows, int vocab) {
-  const int64_t long_tiles = ((int64_t)vocab + kThreads * 32 - 1) / (kThreads * 32);
-  return rows * long_tiles >= 1024 ? 32 : 8;
+  for (int ept = 32; ept > 8; ept /= 2)
+    if (rows * (((int64_t)vocab + kThreads * ept - 1) / (kThreads * ept)) >= kFullCard) return ept;
+  return 8;
 }
 inline int64_t tiles_of(int64_t rows, int vocab) {
   const int64_t n = (int64_t)kThreads * elements_per_thread(rows, vocab);
@@ -442,8 +506,10 @@ int check(int batch, int beams, int vocab, int k, int dtype) {
 
 template <typename T> void launch_part(const PartArgs& a, int ept, int64_t rows, hipStream_t s) {
   const dim3 grid((unsigned)(rows * a.tiles));
-  if (ept == 32) hipLaunchKernelGGL((part_kernel<T, 32>), grid, dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((part_kernel<T, 8>), grid, dim3(kThreads), 0, s, a);
+  const size_t lds = (size_t)a.k * ept * sizeof(uint64_t);
+  if (ept == 32) hipLaunchKernelGGL((part_kernel<T, 32>), grid, dim3(kThreads), lds, s, a);
+  else if (ept == 16) hipLaunchKernelGGL((part_kernel<T, 16>), grid, dim3(kThreads), lds, s, a);
+  else hipLaunchKernelGGL((part_kernel<T, 8>), grid, dim3(kThreads), lds, s, a);
 }
 
 }  // namespace beam
