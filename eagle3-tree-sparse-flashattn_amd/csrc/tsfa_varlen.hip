@@ -90,6 +90,11 @@ __device__ inline void dma_1k(const void* base, uint32_t off, uint32_t lds_in) {
                : "v"(off), "s"(sbase), "s"(lds)
                : "memory", "m0");
 }
+// The same with an address per lane.
+__device__ inline void dma_1k_rows(const void* src, uint32_t lds_in) {
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_in);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
 // N such loads to consecutive LDS KBs from one base: load i reads base +
 // off[i] + i KB (the immediate offset counts for both addresses).
 template <int N> __device__ inline void dma_rows(const void* base, const uint32_t (&off)[N], uint32_t lds_in) {
@@ -203,8 +208,21 @@ template <int D, int S, int RG> struct Shape {
   static constexpr int kLpw = kUnit / 1024 / RG;           // 1 KB loads of a wave per unit
   static constexpr int kRing = S * kStages * kUnit;
   static constexpr int kWords = kTreeUnits * kRows * 4;
+  // Q's way in: its rows fill the last kQStages stages of every ring before
+  // these are first used, so kAhead units are requested beside it
+  static constexpr int kQBytes = kRows * kRowBytes;
+  static constexpr int kQStages = (kQBytes + S * kUnit - 1) / (S * kUnit);
+  static constexpr int kQLoads = kQBytes / 1024 / kWaves;
+  static constexpr int kAhead = kStages - (kQStages > (S == 1 ? 2 : 1) ? kQStages : (S == 1 ? 2 : 1));
   static constexpr int kLds = kRing + kTableIds * 8 + kWords;
 };
+
+// LDS byte of Q's byte x (of a 1 KB load, or a row group's rows): the last
+// kQStages stages of ring 0, then of ring 1, ...
+template <typename C> __device__ inline int q_place(int x) {
+  constexpr int PER = C::kQStages * C::kUnit;
+  return x / PER * (C::kStages * C::kUnit) + (C::kStages - C::kQStages) * C::kUnit + x % PER;
+}
 
 template <typename T, int D, int S, int RG>
 __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
@@ -316,15 +334,6 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     const int t = (int)fdiv((uint32_t)R, cut.by_group), g = R - t * G;
     const float sl2 = a.scale_log2;
 
-    // Q^T operand: lane (ln, lh) holds d = 16 kk + 8 lh + [0, 8) of its row
-    i16x8 qf[KS];
-    {
-      const T* qrow = static_cast<const T*>(a.q) + (int64_t)(sq.q0 + t) * a.sqn + (int64_t)(pl.kvh * G + g) * a.sqh;
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk)
-        qf[kk] = *reinterpret_cast<const i16x8*>(qrow + 16 * kk + 8 * lh) ^ (short)(a.neg_q ? 0x8000 : 0);
-    }
-
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -408,6 +417,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         peek(j + 1);
       };
 
+      i16x8 qf[KS];  // Q^T operand: lane (ln, lh) holds d = 16 kk + 8 lh + [0, 8) of its row
       // S^T of the unit at kt: lane (ln, lh) element i is key 8 (i / 4) + 4 lh
       // + i % 4 of row ln.  K is read KA steps ahead, fenced (left alone, the
       // compiler reads one step ahead and each MFMA waits an LDS latency);
@@ -482,7 +492,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         };
         if constexpr (NEXT) {
           const f32x16 sn = scores(smem + (st * NST + (uint32_t)(j + 1) % NST) * C::kUnit, [&]() {
-            if (issued < n) issue(issued++);
+            while (issued < min(n, j + NST - STAG)) issue(issued++);
             stats();
           }, [&](int kk) {
 #pragma unroll
@@ -567,7 +577,19 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       };
 
       vm_wait<0>();  // the ring's waits count its own loads alone
-      while (issued < NST - 1 - STAG && issued < n) issue(issued++);
+      // Q comes through the rings' last stages, rows whole, in K's layout (16
+      // bytes a lane straight from the rows touch a cache line per lane: 2 us
+      // of a tile's start).
+#pragma unroll 1
+      for (int i = 0; i < C::kQLoads; ++i) {
+        const int row = (wave * C::kQLoads + i) * RPL + lane / CPR;
+        const int rr = min(pl.tile * M + row, TG - 1);
+        const int tt = (int)fdiv((uint32_t)rr, cut.by_group), gg = rr - tt * G;
+        const T* src = static_cast<const T*>(a.q) + (int64_t)(sq.q0 + tt) * a.sqn + (int64_t)(pl.kvh * G + gg) * a.sqh +
+                       (((lane % CPR) ^ swz_k<D>(row)) << 3);
+        dma_1k_rows(src, lds_addr(smem) + q_place<C>((wave * C::kQLoads + i) * 1024));
+      }
+      while (issued < C::kAhead && issued < n) issue(issued++);
       if (a.mask != nullptr) {
         // under the first units' way here; the barriers below order them
         for (int i = tid; i < (c1 * S - ut0) * M; i += C::kWaves * 64) {
@@ -578,6 +600,13 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       int j = 0;
       wait_units<LPW, NST - 2>(issued - 1);
       barrier();
+      {
+        const unsigned char* qt = smem + q_place<C>(rg * 32 * C::kRowBytes) + ln * C::kRowBytes;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+          qf[kk] = *reinterpret_cast<const i16x8*>(qt + (((2 * kk + lh) ^ swz_k<D>(ln)) << 4)) ^
+                   (short)(a.neg_q ? 0x8000 : 0);
+      }
       f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
       uint32_t pk[8], w = 0xffffffffu;
       constexpr std::true_type full{};
@@ -591,7 +620,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         const int n_full = min(n, seen_by_all / (32 * S) - c0);
         const bool late = STAG != 0 && rg >= RG / 2;
         auto meet = [&](int i) {
-          if (issued < n) vm_wait<(NST - 3 - STAG) * LPW>();
+          if (i > 0 && issued < n) vm_wait<(NST - 3 - STAG) * LPW>();  // issued = i + NST - 1 - STAG
           else wait_units<LPW, NST - 3>(issued - 2 - i);
           barrier();
         };

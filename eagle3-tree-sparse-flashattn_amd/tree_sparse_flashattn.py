@@ -1126,10 +1126,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
             _remember(_SELECT_CALLS, key, call)
     dev, strides, shape, row_bytes, pointers, ws_bytes = call
     batch = shape[0]
-    tokens, parents = torch.empty((2, batch, k), dtype=torch.int64, device=dev).unbind(0)
-    best = torch.empty((batch, k), dtype=torch.float32, device=dev)
-    dst = tuple([torch.empty((batch, k, *t.shape[2:]), dtype=t.dtype, device=dev) for t in src])
-    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=dev)
+    tokens, parents = scores.new_empty((2, batch, k), dtype=torch.int64).unbind(0)
+    best = scores.new_empty((batch, k))
+    dst = tuple([t.new_empty((batch, k, *t.shape[2:])) for t in src])
+    ws = scores.new_empty((ws_bytes or 1,), dtype=torch.uint8)
     _run_on(dev, "beam_select", _lib.load().tsfa_beam_select,
             (logits.data_ptr(), strides[0], strides[1], scores.data_ptr(), strides[2], strides[3], *shape,
              tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), pointers(*[t.data_ptr() for t in src]),
