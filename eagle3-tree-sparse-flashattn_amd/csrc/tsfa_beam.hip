@@ -477,9 +477,9 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
 
 // States too large for the merge's one workgroup per sequence.
 __global__ __launch_bounds__(kThreads) void states_kernel(const States st, const int64_t* parents, int beams, int k) {
-  const int at = blockIdx.y;
-  copy_row(st, blockIdx.z, (int64_t)(at / k) * beams + parents[at], at, (int64_t)blockIdx.x * kThreads + threadIdx.x,
-           (int64_t)gridDim.x * kThreads);
+  const int at = blockIdx.x;
+  copy_row(st, blockIdx.z, (int64_t)(at / k) * beams + parents[at], at, (int64_t)blockIdx.y * kThreads + threadIdx.x,
+           (int64_t)gridDim.y * kThreads);
 }
 
 // Elements of a tile per thread: long tiles where they fill the card, short
@@ -500,7 +500,7 @@ int check(int batch, int beams, int vocab, int k, int dtype) {
   if (dtype != TSFA_DTYPE_FP16 && dtype != TSFA_DTYPE_BF16 && dtype != TSFA_DTYPE_FP32) return TSFA_ERR_UNSUPPORTED;
   if (k > kMaxK || beams > kMaxBeams || (int64_t)beams * vocab > (1 << 30)) return TSFA_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)batch * beams;
-  if ((int64_t)batch * k > 65535 || rows * tiles_of(rows, vocab) > INT32_MAX) return TSFA_ERR_UNSUPPORTED;
+  if ((int64_t)batch * k > INT32_MAX || rows * tiles_of(rows, vocab) > INT32_MAX) return TSFA_ERR_UNSUPPORTED;
   return TSFA_OK;
 }
 
@@ -594,7 +594,7 @@ extern "C" int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, i
   hipLaunchKernelGGL(merge_kernel, dim3((unsigned)batch), dim3(kMergeThreads), 0, s, ma);
   if (!inside) {
     const int64_t blocks = (most / 16 + kThreads) / kThreads;
-    hipLaunchKernelGGL(states_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), (unsigned)(batch * k), (unsigned)n_states),
+    hipLaunchKernelGGL(states_kernel, dim3((unsigned)(batch * k), (unsigned)(blocks < 64 ? blocks : 64), (unsigned)n_states),
                        dim3(kThreads), 0, s, sa, (const int64_t*)parents, beams, k);
   }
   return hipGetLastError() == hipSuccess ? TSFA_OK : TSFA_ERR_LAUNCH;

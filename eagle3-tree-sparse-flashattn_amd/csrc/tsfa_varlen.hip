@@ -928,7 +928,7 @@ inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv
   const int64_t rows = (int64_t)total_q * (num_heads / num_kv_heads);
   s.rows = rows <= (int64_t)32 * batch ? 32 : rows > (int64_t)512 * batch ? 256 : 128;
   s.streams = s.rows == 32 ? 4 : s.rows == 256 ? 1 : 2;
-  s.extra = s.rows == 32 ? 3 : s.rows == 256 ? 8 : 8;
+  s.extra = s.rows == 32 ? 2 : 8;
   s.groups = cus < kMaxGroups ? cus : kMaxGroups;
   s.o = align256((size_t)2 * s.groups * s.rows * head_dim * 4);
   s.ml = align256((size_t)2 * s.groups * s.rows * 8);

@@ -876,6 +876,7 @@ def append_paged_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache:
     tokens must not share a place.  No host synchronisation; nothing about the
     lengths is checked on the host.
     """
+    interleaved, attention_scaling = bool(interleaved), float(attention_scaling)
     # a geometry that ran as given (no copies) skips the checks its first call
     # made; everything they look at but the pointers is in the key
     key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), kv_cache.shape, kv_cache.stride(),
@@ -959,7 +960,7 @@ def _append_plan(q, k, v, kv_cache, kv_indices, positions, inv_freq, q_indptr, k
         q = q.contiguous()
         dst = q
     strides = _lib.i64_array((*q.stride(), *k.stride(), *v.stride(), *dst.stride()))
-    rotation = (int(positions.dtype == torch.int64), 2 * inv_freq.numel(), int(interleaved), float(attention_scaling))
+    rotation = (int(positions.dtype == torch.int64), 2 * inv_freq.numel(), int(interleaved), attention_scaling)
     lists = (_table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size)
     tail = (strides, _lib.i64_array(cache_strides), batch, n, n_heads, n_kv_heads, head_dim, dt)
     operands = (q, k, v, kv_indices, positions, inv_freq, q_indptr, kv_lens, kv_indptr)
@@ -986,13 +987,15 @@ def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tens
     O [N, Hq, D] in q's dtype; with ``return_lse`` ``(O, lse)``, lse [N, Hq]
     float32.  A row that sees no key is 0 (its lse -inf): the uniform forwards
     return NaN there, as the reference does, but here such rows pad a batch
-    and would carry the NaN into the cache.  Rows behind q_indptr[B] are left
-    as they were.  ``workspace`` (uint8,
+    and would carry the NaN into the cache.  Rows of ``out`` behind
+    q_indptr[B] are left as they were (those of lse are not set).  Sequences
+    may share pages.  ``workspace`` (uint8,
     fwd_paged_varlen_workspace_bytes(...) bytes) must not be shared by calls
     that overlap in time, captured graphs among them.  No host
     synchronisation; page ids outside the pool are clamped (wrong O, never an
     invalid read).
     """
+    sm_scale = None if sm_scale is None else float(sm_scale)
     key = (q.shape, q.stride(), kv_cache.shape, kv_cache.stride(), kv_indices.shape, kv_indices.stride(),
            q_indptr.shape, q_indptr.stride(), kv_lens.shape, kv_lens.stride(),
            None if kv_indptr is None else (kv_indptr.shape, kv_indptr.stride(), kv_indptr.dtype,
@@ -1065,7 +1068,7 @@ def _varlen_plan(q, kv_cache, kv_indices, tree_mask, q_indptr, kv_lens, kv_indpt
     shape = (batch, n, n_heads, n_kv_heads, head_dim, dt)
     lists = (_table_entries(kv_indices), pt_stride, pt_width, n_pages, page_size)
     tail = (_lib.i64_array(q.stride()), _lib.i64_array(cache_strides), _lib.i64_array(dst.stride()),
-            float(1.0 / math.sqrt(head_dim) if sm_scale is None else sm_scale), *shape)
+            1.0 / math.sqrt(head_dim) if sm_scale is None else sm_scale, *shape)
     operands = (q, kv_indices, mask, q_indptr, kv_lens, kv_indptr)
     return ((dev, mask_args, lists, tail, _varlen_workspace_bytes(dev, shape), copy_out),
             all(x is y for x, y in zip(given, operands)), operands)
@@ -1115,6 +1118,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
     A draft's tree grows by ``parents``: continuation j of this step is a child
     of continuation parents[b, j] of the step before.
     """
+    k = int(k)
     key = (logits.shape, logits.stride(), logits.dtype, logits.get_device(), scores.shape, scores.stride(),
            scores.dtype, scores.get_device(), k,
            tuple([(t.shape, t.stride(), t.dtype, t.get_device()) for t in states]))

@@ -311,7 +311,7 @@ int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* o, float* l
  * states     n_states (at most 8) host pointers to [batch, beams] dense rows
  *            of state_row_bytes bytes, copied to out_states [batch, k]
  * Supported: k <= 64 (and <= beams * vocab), beams <= 256, beams * vocab <=
- * 2^30, batch * k <= 65535.  workspace 16-byte aligned. */
+ * 2^30.  workspace 16-byte aligned. */
 size_t tsfa_beam_select_workspace_bytes(int batch, int beams, int vocab, int k);
 int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, int64_t logits_beam_stride,
                      const float* scores, int64_t scores_seq_stride, int64_t scores_beam_stride, int batch,

@@ -84,7 +84,11 @@ ATTEND = [
     ([8, 8], [208, 1008], dict(hq=4, hkv=4)),                                # few rows, 32-row tiles
     ([2] * 70, [3 + 13 * i % 200 for i in range(70)], dict(hq=4, hkv=2, d=64, mask="causal")),  # above 64 sequences
     ([600], [650], dict(hq=2, hkv=2, d=64)),                                 # words of a wide tree in several parts
-    ([1], [17000], dict(hq=2, hkv=1, d=64, mask="causal")),                  # a page list in several parts
+    ([1], [17000], dict(hq=2, hkv=1, d=64, mask="causal")),                  # a long page list
+    ([1, 2], [5000, 2300], dict()),                                          # 32-row tiles, many steps
+    ([40], [2100], dict(dtype=FP)),                                          # 128-row tiles, many steps
+    ([150, 140], [1050, 1640], dict(hq=8, hkv=1)),                           # 256-row tiles, many steps
+    ([90], [700], dict(hq=8, hkv=1, d=64, mask="causal", layout="HND")),
 ]
 
 
@@ -94,6 +98,48 @@ def test_varlen_attention(case):
     print(f"[attend] {q_lens} {kv_lens} {kw}", flush=True)
     # rows of the pool that hold no key are NaN: none may reach a result
     _attend(q_lens, [max(a, b) for a, b in zip(q_lens, kv_lens)], seed=len(q_lens), **kw)
+
+
+# kv heads, query heads per kv head, query tokens, keys, batch: every workgroup walks more keys than its table of
+# pages of 16 keys holds (the three tile shapes), or more of a tree than its table of visibility words
+LONG = [(16, 8, 512, 17000, 1), (16, 4, 30, 17000, 16), (16, 1, 1, 40000, 8), (16, 8, 700, 760, 1)]
+
+
+@pytest.mark.parametrize("case", LONG, ids=[f"l{i}" for i in range(len(LONG))])
+def test_varlen_runs_longer_than_their_tables(case):
+    hkv, group, q_len, keys, batch = case
+    print(f"[attend] {case}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(q_len)
+    d, n = 64, batch * q_len
+    q = torch.randn(n, hkv * group, d, generator=g, device="cuda").to(BF)
+    kv = torch.randn(batch, 2, hkv, keys, d, generator=g, device="cuda").to(BF)
+    mask = su.tree_masks([q_len])[0].cuda()
+    lens = dict(q_indptr=torch.arange(batch + 1, dtype=torch.int32, device="cuda") * q_len,
+                kv_lens=torch.full((batch,), keys, dtype=torch.int32, device="cuda"))
+    outs = []
+    for page in (16, 1024):
+        pages = -(-keys // page)
+        cache = torch.zeros(batch, 2, hkv, pages * page, d, dtype=BF, device="cuda")
+        cache[:, :, :, :keys] = kv
+        cache = cache.view(batch, 2, hkv, pages, page, d).permute(0, 3, 1, 2, 4, 5).reshape(-1, 2, hkv, page, d)
+        table = torch.arange(batch * pages, dtype=torch.int32, device="cuda").view(batch, pages)
+        outs.append(tsf.tree_sparse_attention_fwd_paged_varlen(q, cache, table, mask, kv_layout="HND", **lens))
+        del cache
+    torch.cuda.synchronize()
+    # the pages' size changes where a run's tables end and nothing else
+    assert torch.equal(outs[0], outs[1])
+    # the last sequence's first and last kv head in 64 bits
+    for h in (0, hkv - 1):
+        k, v = kv[-1, 0, h].double(), kv[-1, 1, h].double()
+        x = q[n - q_len:, h * group:(h + 1) * group].double().transpose(0, 1).reshape(-1, d)
+        score = (x @ k.t()) * d ** -0.5
+        most = float((x.abs() @ k.abs().t()).max()) * d ** -0.5
+        score = score.view(group, q_len, keys)
+        score[:, :, keys - q_len:].masked_fill_(~mask, -torch.inf)
+        w = torch.softmax(score, -1).view(-1, keys)
+        ref, size = w @ v, w @ v.abs()
+        got = outs[0][n - q_len:, h * group:(h + 1) * group].double().transpose(0, 1).reshape(-1, d)
+        assert bool(((got - ref).abs() <= so.attention_tolerance(ref, size, most, BF, keys)).all())
 
 
 @pytest.mark.parametrize("sm_scale", [0.0, -0.2, 3.0])
@@ -251,6 +297,41 @@ def test_varlen_graph_follows_the_lengths():
             g.replay()
             torch.cuda.synchronize()
             assert _same(out[:rows[-1]], eager[:rows[-1]])
+
+
+def test_varlen_shared_and_repeated_pages():
+    print("[attend] pages shared by sequences, and twice in one list", flush=True)
+
+    def edit(q, cache, lists, tree):
+        lists[1][:4] = lists[0][:4]  # a common prefix
+        lists[2][3] = lists[2][1]
+
+    _attend([9, 20, 3], [105, 90, 80], edit=edit, stale=None)
+
+
+def test_varlen_and_append_in_a_pool_past_32_bit_offsets():
+    print("[attend] a pool of more than 2^31 elements", flush=True)
+    q_lens, kv_lens, hkv, d = [17, 1], [200, 33], 8, 128
+    g = torch.Generator().manual_seed(2)
+    small, lists = su.pool(q_lens, kv_lens, hkv, d, BF, 16)
+    n, total = small.shape[0], (1 << 31) // (2 * 16 * hkv * d) + 100
+    big = torch.empty((total, 2, 16, hkv, d), dtype=BF, device="cuda")
+    assert big.numel() > 1 << 31
+    big[total - n:] = small.cuda()
+    qkv = torch.randn(18, 32 + 2 * hkv, d, generator=g).to(BF).cuda()
+    freq, positions = su.inv_freq(d).cuda(), torch.arange(18).cuda()
+    outs = []
+    for cache, shift in ((small.cuda(), 0), (big, total - n)):
+        indices, indptr = su.tables([[p + shift for p in x] for x in lists])
+        q_indptr, kl = su.lengths(q_lens, kv_lens)
+        kw = dict(q_indptr=q_indptr.cuda(), kv_lens=kl.cuda(), kv_indptr=indptr.cuda())
+        q = tsf.append_paged_kv(qkv[:, :32], qkv[:, 32:32 + hkv], qkv[:, 32 + hkv:], cache, indices.cuda(), positions,
+                                freq, **kw)
+        o = tsf.tree_sparse_attention_fwd_paged_varlen(q, cache, indices.cuda(), su.tree_masks(q_lens).cuda(), **kw)
+        outs.append((q, o, cache[-n:]))
+    torch.cuda.synchronize()
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
 
 
 def test_varlen_two_streams_at_once():
@@ -411,6 +492,33 @@ def test_select_ties_and_masked_vocabularies(dtype):
     scores[5, 0] = -inf
     _select(logits, scores, 20)
     _select(logits[:, :1].contiguous(), scores[:, :1].contiguous(), 64)
+
+
+def test_select_more_ties_than_a_round_holds():
+    print("[select] ties across beams", flush=True)
+    logits = torch.full((2, 64, 2100), 0.25, dtype=BF)
+    scores = torch.full((2, 64), -1.0)
+    logits[1, 5:, 7] = 3.0  # and ties at the top
+    _select(logits, scores, 64)
+
+
+def test_select_logits_past_32_bit_offsets():
+    print("[select] logits of more than 2^31 elements apart", flush=True)
+    logits, scores = _logits(2, 3, 5000, BF, seed=8)
+    want = _select(logits, scores, 12)
+    memory = torch.empty(((1 << 31) + 40000,), dtype=BF, device="cuda")
+    far = memory.as_strided((2, 3, 5000), ((1 << 31) + 64, 5001, 1))
+    far.copy_(logits)
+    got = tsf.beam_select(far, scores.cuda(), 12)
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a, b)
+
+
+def test_select_states_moved_by_a_launch_of_their_own():
+    print("[select] large states", flush=True)
+    logits, scores = _logits(3, 4, 300, FP, seed=5)
+    g = torch.Generator().manual_seed(3)
+    _select(logits, scores, 9, (torch.randn(3, 4, 40001, generator=g), torch.randint(9, (3, 4, 7), generator=g)))
 
 
 def test_select_strides_and_empty_batches():

@@ -178,7 +178,7 @@ def test_c_append_checks(kw, status):
     (dict(beams=300), _lib.TSFA_ERR_UNSUPPORTED),
     (dict(beams=2, vocab=3, k=7), _lib.TSFA_ERR_INVALID_ARGUMENT),
     (dict(vocab=1 << 30), _lib.TSFA_ERR_UNSUPPORTED),
-    (dict(batch=20000), _lib.TSFA_ERR_UNSUPPORTED),                   # batch * k rows of states
+    (dict(batch=1 << 30), _lib.TSFA_ERR_UNSUPPORTED),                 # batch * k rows of states
     (dict(dtype=7), _lib.TSFA_ERR_UNSUPPORTED),
     (dict(n_states=9), _lib.TSFA_ERR_UNSUPPORTED),
     (dict(n_states=-1), _lib.TSFA_ERR_INVALID_ARGUMENT),
