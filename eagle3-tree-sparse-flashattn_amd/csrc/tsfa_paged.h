@@ -32,7 +32,7 @@ struct Seq {
   int q0, q_len;   // query rows
   int kv_len;      // keys, at most what the list's pages hold
   int prefix;      // keys before the query tokens' own
-  int64_t list;    // first entry of the page list in kv_indices
+  int list;        // first entry of the page list in kv_indices (of 2^31 - 1 at most)
   int pages;       // entries of the list
 };
 
@@ -43,10 +43,10 @@ TSFA_HD inline Seq seq_of(const Seqs& s, int b) {
   r.q0 = (int)clamp64(s.q_indptr[b], 0, s.total_q);
   r.q_len = (int)clamp64(s.q_indptr[b + 1], r.q0, s.total_q) - r.q0;
   if (s.kv_indptr != nullptr) {
-    r.list = clamp64(s.kv_indptr[b], 0, s.n_indices);
+    r.list = (int)clamp64(s.kv_indptr[b], 0, s.n_indices);
     r.pages = (int)(clamp64(s.kv_indptr[b + 1], r.list, s.n_indices) - r.list);
   } else {
-    r.list = (int64_t)b * s.pt_stride;
+    r.list = (int)(b * s.pt_stride);
     r.pages = s.pt_width;
   }
   const int64_t held = (int64_t)r.pages << s.page_shift;
@@ -84,6 +84,17 @@ struct Cut {
   int extra;                // steps that a tile's start and end cost
 };
 
+// 1 / d to 2^-48: on the device the hardware's estimate and one Newton step (a
+// full division is three times the instructions, on every call's first path).
+TSFA_HD inline double inverse(int64_t d) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const double x = (double)d, r = __builtin_amdgcn_rcp(x);
+  return __builtin_fma(r, __builtin_fma(-x, r, 1.0), r);
+#else
+  return 1.0 / (double)d;
+#endif
+}
+
 inline Cut make_cut(int rows, int keys, int group, int num_kv_heads, int causal, int extra) {
   Cut c;
   c.rows = rows;
@@ -95,17 +106,21 @@ inline Cut make_cut(int rows, int keys, int group, int num_kv_heads, int causal,
   for (c.rows_shift = 0; (1 << c.rows_shift) < rows;) ++c.rows_shift;
   c.by_group = make_fastdiv((uint32_t)group);
   c.unit = (int64_t)keys * group;
-  c.inv_unit = 1.0 / (double)c.unit;
+  c.inv_unit = inverse(c.unit);
   c.extra = extra;
   return c;
 }
 
-// x / d for 0 <= x < 2^52, inv = 1 / d: off by one at most before the remainder is looked at.
+// x / d for 0 <= x < 2^52, inv = inverse(d).  Below 2^30 the half keeps (x +
+// 1/2) / d at least 1/2 / d from a whole number, more than the 2^-18 that the
+// product is off; above, the quotient is off by one at most before the
+// remainder is looked at (2^52 2^-48 / d: by 16 / d).
 TSFA_HD inline int64_t udiv(int64_t x, int64_t d, double inv) {
+  if (x < (1 << 30)) return (int)(((double)(int)x + 0.5) * inv);
   int64_t q = (int64_t)((double)x * inv);
-  const int64_t r = x - q * d;
-  if (r < 0) --q;
-  else if (r >= d) ++q;
+  int64_t r = x - q * d;
+  for (; r < 0; r += d) --q;
+  for (; r >= d; r -= d) ++q;
   return q;
 }
 
@@ -150,15 +165,16 @@ TSFA_HD inline Place place_in_seq(const Cut& c, const Seq& s, int64_t x) {
   Place p;
   const int n = cut_tiles(c, s);
   const int64_t head = head_length(c, s);
-  p.kvh = (int)udiv(x, head, 1.0 / (double)head);
+  p.kvh = (int)udiv(x, head, inverse(head));
   x -= p.kvh * head;
   const int64_t a = tile_first(c, s);
   if (!c.causal) {
-    p.tile = (int)udiv(x, a, 1.0 / (double)a);
+    p.tile = (int)udiv(x, a, inverse(a));
   } else {
-    // the last r with r a + rows r (r - 1) / 2 <= x
-    const double h = (double)a - 0.5 * c.rows;
-    int64_t r = (int64_t)((__builtin_sqrt(h * h + 2.0 * c.rows * (double)x) - h) / c.rows);
+    // the last r with r a + rows r (r - 1) / 2 <= x: the root of the quadratic
+    // with equality, taken in 32 bits and then looked at
+    const float h = (float)a - 0.5f * c.rows, y = 2.0f * (float)x;
+    int64_t r = (int64_t)(y / (h + __builtin_sqrtf(h * h + c.rows * y)));
     r = clamp64(r, 0, n - 1);
     while (r > 0 && tiles_length(c, s, r) > x) --r;
     while (r + 1 < n && tiles_length(c, s, r + 1) <= x) ++r;
@@ -180,7 +196,7 @@ TSFA_HD inline Place place_in_seq(const Cut& c, const Seq& s, int64_t x) {
 // Length of a run, at least half a step's: with fewer steps than workgroups a
 // run holds one step or none.
 TSFA_HD inline int64_t run_length(const Cut& c, int64_t total, int groups) {
-  const int64_t per = udiv(total + groups - 1, groups, 1.0 / (double)groups);
+  const int64_t per = udiv(total + groups - 1, groups, inverse(groups));
   return per > (c.unit + 1) / 2 ? per : (c.unit + 1) / 2;
 }
 // Steps of a tile that start before the line's point `ahead` past its start.

@@ -57,11 +57,11 @@ struct Args {
   int num_heads, groups;           // workgroups on the line
   float4* ws_o;                    // [2 * groups][RG][D / 8][64] unnormalised O, a lane's registers in order
   float2* ws_ml;                   // [2 * groups][rows] (m, l)
-  // [groups] the tile that starts in the run and ends behind it: sequence, kv
-  // head, tile and how many runs on it ends (0: none), its place on the line,
-  // a run's length
+  int* ws_runs;                    // [groups] runs on which the tile that starts in the run ends (0: within it)
+  // [groups] that tile: its sequence's query rows, kv head, tile, place on the
+  // line, a run's length
   struct Desc {
-    int b, kvh, tile, runs;
+    int q0, q_len, kvh, tile;
     int64_t at, per;
   };
   Desc* ws_desc;
@@ -173,21 +173,26 @@ __device__ inline int64_t lane_scan(int64_t x) {
 // The sequences in a wave's registers, lane l holding sequence b0 + l.
 struct LaneSeqs {
   int b0;
-  Seq mine;
-  __device__ void load(const paged::Seqs& s, int from, int lane) {
+  int q0, q_len, kv_len, list;
+  // loads and returns the line up to and including each lane's sequence
+  __device__ int64_t load(const paged::Seqs& s, const Cut& c, int from, int lane) {
     b0 = from;
-    mine = Seq{};
+    Seq mine{};
     if (b0 + lane < s.batch) mine = paged::seq_of(s, b0 + lane);
+    q0 = mine.q0;
+    q_len = mine.q_len;
+    kv_len = mine.kv_len;
+    list = mine.list;
+    return lane_scan(paged::head_length(c, mine) * c.num_kv_heads);
   }
-  __device__ int64_t length(const Cut& c) const { return paged::head_length(c, mine) * c.num_kv_heads; }
   __device__ Seq at(int l) const {
     Seq r;
-    r.q0 = __builtin_amdgcn_readlane(mine.q0, l);
-    r.q_len = __builtin_amdgcn_readlane(mine.q_len, l);
-    r.kv_len = __builtin_amdgcn_readlane(mine.kv_len, l);
-    r.prefix = __builtin_amdgcn_readlane(mine.prefix, l);
-    r.list = readlane64(mine.list, l);
-    r.pages = __builtin_amdgcn_readlane(mine.pages, l);
+    r.q0 = __builtin_amdgcn_readlane(q0, l);
+    r.q_len = __builtin_amdgcn_readlane(q_len, l);
+    r.kv_len = __builtin_amdgcn_readlane(kv_len, l);
+    r.prefix = max(r.kv_len - r.q_len, 0);
+    r.list = __builtin_amdgcn_readlane(list, l);
+    r.pages = 0;  // kv_len lies within them
     return r;
   }
 };
@@ -254,17 +259,13 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   const int G = cut.group;
 
   const int run = run_of_block(blockIdx.x, a.groups);
-  if (tid == 0) a.ws_desc[run].runs = 0;
+  if (tid == 0) a.ws_runs[run] = 0;
   LaneSeqs seqs;
-  seqs.load(a.seqs, 0, lane);
-  int64_t upto = lane_scan(seqs.length(cut));  // of chunk 0
+  int64_t upto = seqs.load(a.seqs, cut, 0, lane);  // of the chunk in registers
   int64_t total = readlane64(upto, 63);
   if (a.seqs.batch > 64) {
-    for (int b0 = 64; b0 < a.seqs.batch; b0 += 64) {
-      seqs.load(a.seqs, b0, lane);
-      total += readlane64(lane_scan(seqs.length(cut)), 63);
-    }
-    seqs.load(a.seqs, 0, lane);
+    for (int b0 = 64; b0 < a.seqs.batch; b0 += 64) total += readlane64(seqs.load(a.seqs, cut, b0, lane), 63);
+    upto = seqs.load(a.seqs, cut, 0, lane);
   }
   const int64_t per = uniform64(paged::run_length(cut, total, a.groups));
   int64_t at = run * per;  // the run: [at, end) of the line
@@ -274,8 +275,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
   while (before + readlane64(upto, 63) <= at) {
     before += readlane64(upto, 63);
     if (seqs.b0 + 64 >= a.seqs.batch) return;  // not reached: at < total
-    seqs.load(a.seqs, seqs.b0 + 64, lane);
-    upto = lane_scan(seqs.length(cut));
+    upto = seqs.load(a.seqs, cut, seqs.b0 + 64, lane);
   }
   int sl = __builtin_ctzll(__ballot(before + upto > at));
   Seq sq = seqs.at(sl);
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     do {
       if (seqs.b0 + ++sl >= a.seqs.batch) return false;
       if (sl == 64) {
-        seqs.load(a.seqs, seqs.b0 + 64, lane);
+        seqs.load(a.seqs, cut, seqs.b0 + 64, lane);
         sl = 0;
       }
       sq = seqs.at(sl);
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         }
       };
 
-      vm_wait<0>();  // the ring's waits count its own loads alone
+      vm_wait<0>();  // the ring's waits count its own loads and Q's alone
       // Q comes through the rings' last stages, rows whole, in K's layout (16
       // bytes a lane straight from the rows touch a cache line per lane: 2 us
       // of a tile's start).
@@ -743,8 +743,9 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     }
     if (tid == 0 && s0 == 0 && s1 < n_steps) {
       const int64_t tile_at = end - left;  // the run that the tile's last step starts in:
-      const int64_t last = paged::udiv(tile_at + (n_steps - 1) * cut.unit, per, 1.0 / (double)per);
-      a.ws_desc[run] = Args::Desc{b, pl.kvh, pl.tile, (int)(last - run) + 1, tile_at, per};
+      const int64_t last = paged::udiv(tile_at + (n_steps - 1) * cut.unit, per, paged::inverse(per));
+      a.ws_runs[run] = (int)(last - run) + 1;
+      a.ws_desc[run] = Args::Desc{sq.q0, sq.q_len, pl.kvh, pl.tile, tile_at, per};
     }
 
     // on along the line
@@ -770,24 +771,23 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
 // block per run would leave most of them empty and the others few: 17 us against
 // 6 for 16 tiles in 14 parts each.)
 constexpr int kJoin = 4;
-constexpr int kMaxGroups = 1024;
+constexpr int kMaxGroups = 1024;  // a run's number takes 10 bits
 
 // Parts p0, p0 + step, ... of a lane's row and d tile, joined into (m, l, o).
 template <int D, int RG>
-__device__ inline void join_parts(const Args& a, const Args::Desc& desc, int run, int rg, int dt, int p0, int step,
-                                  int lane, float& m, float& l, float4 (&o)[4]) {
+__device__ inline void join_parts(const Args& a, const Args::Desc& desc, int run, int runs, int rg, int dt, int p0,
+                                  int step, int lane, float& m, float& l, float4 (&o)[4]) {
   constexpr int M = 32 * RG;
   const float sl2 = a.scale_log2;
-  for (; p0 < desc.runs; p0 += step * kJoin) {
+  for (; p0 < runs; p0 += step * kJoin) {
     float2 x[kJoin];
     float4 v[kJoin][4];
     bool has[kJoin];
 #pragma unroll
     for (int k = 0; k < kJoin; ++k) {
       // past the last and runs without a step of the tile: loaded, not used
-      const int p = min(p0 + step * k, desc.runs - 1);
-      has[k] = p0 + step * k < desc.runs &&
-               paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
+      const int p = min(p0 + step * k, runs - 1);
+      has[k] = p0 + step * k < runs && paged::run_has_step(a.cut, (int64_t)(run + p) * desc.per, desc.per, desc.at);
       const int64_t slot = p == 0 ? 2 * (int64_t)run + 1 : 2 * (int64_t)(run + p);
       x[k] = a.ws_ml[slot * M + rg * 32 + (lane & 31)];
       const float4* wo = a.ws_o + ((slot * RG + rg) * (D / 8) + 4 * dt) * 64 + lane;
@@ -826,7 +826,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   constexpr int DT = D / 32, PS = 4, M = 32 * RG;
   __shared__ float4 jo[PS * 4 * 64];
   __shared__ float2 jml[PS * 64];
-  __shared__ short tiles[kMaxGroups];
+  __shared__ int tiles[kMaxGroups];  // run and, above, how many it goes on for
   __shared__ int wave_count[kMaxGroups / 64];
   __shared__ int any_long;
   const int lane = threadIdx.x & 63, ps = threadIdx.x >> 6;
@@ -834,7 +834,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   if (threadIdx.x == 0) any_long = 0;
   __syncthreads();
   for (int r0 = ps * 64; r0 < a.groups; r0 += 256) {
-    const int runs = r0 + lane < a.groups ? a.ws_desc[r0 + lane].runs : 0;
+    const int runs = r0 + lane < a.groups ? a.ws_runs[r0 + lane] : 0;
     const uint64_t set = __ballot(runs != 0);
     if (lane == 0) wave_count[r0 / 64] = __builtin_popcountll(set);
     if (runs > kJoin) any_long = 1;
@@ -845,48 +845,46 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
   const int n_items = n_tiles * RG * DT;
   if ((int)blockIdx.x >= n_items) return;
   for (int r0 = ps * 64; r0 < a.groups; r0 += 256) {
-    const bool on = r0 + lane < a.groups && a.ws_desc[r0 + lane].runs != 0;
-    const uint64_t set = __ballot(on);
-    int at = __builtin_popcountll(set & ((1ull << lane) - 1));
+    const int runs = r0 + lane < a.groups ? a.ws_runs[r0 + lane] : 0;
+    int at = __builtin_popcountll(__ballot(runs != 0) & ((1ull << lane) - 1));
     for (int w = 0; w < r0 / 64; ++w) at += wave_count[w];
-    if (on) tiles[at] = (short)(r0 + lane);
+    if (runs != 0) tiles[at] = (runs << 10) | (r0 + lane);
   }
   __syncthreads();
   const float sl2 = a.scale_log2;
   // float4 x of the lane's row and d tile: normalised, rounded and written
-  auto put = [&](const Args::Desc& desc, const Seq& sq, int rg, int dt, int x, float4 r, float m, float l) {
+  auto put = [&](const Args::Desc& desc, int rg, int dt, int x, float4 r, float m, float l) {
     const int G = a.cut.group, row = desc.tile * M + rg * 32 + ln;
-    if (row >= sq.q_len * G) return;
+    if (row >= desc.q_len * G) return;
     const int t = (int)fdiv((uint32_t)row, a.cut.by_group), h = desc.kvh * G + (row - t * G);
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     const T4 v = {(T)(r.x * inv), (T)(r.y * inv), (T)(r.z * inv), (T)(r.w * inv)};
-    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt +
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (int64_t)(desc.q0 + t) * a.son + (int64_t)h * a.soh + 32 * dt +
                            8 * x + 4 * lh) = v;
     if (a.lse != nullptr && dt == 0 && x == 0 && lh == 0)
-      a.lse[(int64_t)(sq.q0 + t) * a.num_heads + h] = l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
+      a.lse[(int64_t)(desc.q0 + t) * a.num_heads + h] =
+          l == 0.f ? -INFINITY : m * (sl2 * 0.6931471805599453f) + logf(l);
   };
   for (int item = blockIdx.x * PS + ps; item < n_items; item += gridDim.x * PS) {
-    const int run = tiles[item / (RG * DT)], rg = item / DT % RG, dt = item % DT;
+    const int tile = __builtin_amdgcn_readfirstlane(tiles[item / (RG * DT)]);
+    const int run = tile & (kMaxGroups - 1), runs = tile >> 10, rg = item / DT % RG, dt = item % DT;
     const Args::Desc desc = a.ws_desc[run];
-    if (desc.runs > kJoin) continue;
-    const Seq sq = paged::seq_of(a.seqs, desc.b);
-    if (desc.tile * M + rg * 32 >= sq.q_len * a.cut.group) continue;
+    if (runs > kJoin || desc.tile * M + rg * 32 >= desc.q_len * a.cut.group) continue;
     float m = -INFINITY, l = 0.f;
     float4 o[4] = {};
-    join_parts<D, RG>(a, desc, run, rg, dt, 0, 1, lane, m, l, o);
+    join_parts<D, RG>(a, desc, run, runs, rg, dt, 0, 1, lane, m, l, o);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) put(desc, sq, rg, dt, x, o[x], m, l);
+    for (int x = 0; x < 4; ++x) put(desc, rg, dt, x, o[x], m, l);
   }
   if (any_long == 0) return;
   for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-    const int run = tiles[item / (RG * DT)], rg = item / DT % RG, dt = item % DT;
+    const int tile = __builtin_amdgcn_readfirstlane(tiles[item / (RG * DT)]);
+    const int run = tile & (kMaxGroups - 1), runs = tile >> 10, rg = item / DT % RG, dt = item % DT;
     const Args::Desc desc = a.ws_desc[run];
-    if (desc.runs <= kJoin) continue;
-    const Seq sq = paged::seq_of(a.seqs, desc.b);
-    if (desc.tile * M + rg * 32 >= sq.q_len * a.cut.group) continue;
+    if (runs <= kJoin || desc.tile * M + rg * 32 >= desc.q_len * a.cut.group) continue;
     float m = -INFINITY, l = 0.f;
     float4 o[4] = {};
-    join_parts<D, RG>(a, desc, run, rg, dt, ps, PS, lane, m, l, o);
+    join_parts<D, RG>(a, desc, run, runs, rg, dt, ps, PS, lane, m, l, o);
     jml[ps * 64 + lane] = make_float2(m, l);
 #pragma unroll
     for (int i = 0; i < 4; ++i) jo[(ps * 4 + i) * 64 + lane] = o[i];
@@ -909,15 +907,15 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
       r.z += v.z * f;
       r.w += v.w * f;
     }
-    put(desc, sq, rg, dt, ps, r, m, l);
+    put(desc, rg, dt, ps, r, m, l);
     __syncthreads();  // jo and jml are written again
   }
 }
 
 struct Sizes {
   int groups, rows, streams, extra;
-  size_t o, ml, desc;
-  size_t total() const { return o + ml + desc; }
+  size_t o, ml, runs, desc;
+  size_t total() const { return o + ml + runs + desc; }
 };
 
 // Tiles by the rows (query token x head of a kv head) of a sequence on
@@ -932,6 +930,7 @@ inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv
   s.groups = cus < kMaxGroups ? cus : kMaxGroups;
   s.o = align256((size_t)2 * s.groups * s.rows * head_dim * 4);
   s.ml = align256((size_t)2 * s.groups * s.rows * 8);
+  s.runs = align256((size_t)s.groups * 4);
   s.desc = align256((size_t)s.groups * sizeof(Args::Desc));
   return s;
 }
@@ -1041,7 +1040,8 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
   char* ws = static_cast<char*>(workspace);
   a.ws_o = reinterpret_cast<float4*>(ws);
   a.ws_ml = reinterpret_cast<float2*>(ws + sz.o);
-  a.ws_desc = reinterpret_cast<varlen::Args::Desc*>(ws + sz.o + sz.ml);
+  a.ws_runs = reinterpret_cast<int*>(ws + sz.o + sz.ml);
+  a.ws_desc = reinterpret_cast<varlen::Args::Desc*>(ws + sz.o + sz.ml + sz.runs);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == TSFA_DTYPE_BF16)
     return head_dim == 128 ? varlen::launch_tiles<__bf16, 128>(a, sz.rows, s) : varlen::launch_tiles<__bf16, 64>(a, sz.rows, s);

@@ -23,7 +23,21 @@ using namespace tsfa::paged;
   } while (0)
 static int g_case = 0;
 
+static void check_udiv(std::mt19937_64& rng) {
+  for (int i = 0; i < 2000000; ++i) {
+    const int64_t d = 1 + (int64_t)(rng() >> (24 + rng() % 40));
+    int64_t x = (int64_t)(rng() >> (12 + rng() % 52));
+    if (i % 3 == 0) x = x / d * d;          // at a multiple, and just below one
+    if (i % 3 == 1) x = x / d * d + d - 1;
+    if (x < 0 || x >= ((int64_t)1 << 52)) continue;
+    // the device's inverse is up to 2^-48 off either way
+    for (double e : {0.0, 3.5e-15, -3.5e-15}) CHECK(udiv(x, d, inverse(d) * (1 + e)) == x / d);
+  }
+}
+
 int main() {
+  std::mt19937_64 rng64(3);
+  check_udiv(rng64);
   std::mt19937 rng(7);
   auto pick = [&](int lo, int hi) { return (int)(lo + rng() % (uint32_t)(hi - lo + 1)); };
   for (g_case = 0; g_case < 3000; ++g_case) {
@@ -162,7 +176,7 @@ int main() {
           CHECK(held == v.size());
           // the number of parts as the first run writes it for the join
           if (v.size() > 1)
-            CHECK((int)udiv(line + (n - 1) * c.unit, per, 1.0 / per) == std::get<0>(v.back()));
+            CHECK((int)udiv(line + (n - 1) * c.unit, per, inverse(per)) == std::get<0>(v.back()));
           line += tile_first(c, q) + tile_more(c) * t;
         }
     }
