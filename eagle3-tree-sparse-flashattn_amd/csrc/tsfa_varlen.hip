@@ -607,6 +607,11 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           qf[kk] = *reinterpret_cast<const i16x8*>(qt + (((2 * kk + lh) ^ swz_k<D>(ln)) << 4)) ^
                    (short)(a.neg_q ? 0x8000 : 0);
       }
+      if constexpr (C::kAhead < 2) {
+        // unit 1 takes Q's stage: it has to be on its way before step 1 waits
+        barrier();
+        while (issued < min(n, NST)) issue(issued++);
+      }
       f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
       uint32_t pk[8], w = 0xffffffffu;
       constexpr std::true_type full{};

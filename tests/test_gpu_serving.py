@@ -100,46 +100,52 @@ def test_varlen_attention(case):
     _attend(q_lens, [max(a, b) for a, b in zip(q_lens, kv_lens)], seed=len(q_lens), **kw)
 
 
-# kv heads, query heads per kv head, query tokens, keys, batch: every workgroup walks more keys than its table of
-# pages of 16 keys holds (the three tile shapes), or more of a tree than its table of visibility words
-LONG = [(16, 8, 512, 17000, 1), (16, 4, 30, 17000, 16), (16, 1, 1, 40000, 8), (16, 8, 700, 760, 1)]
+# kv heads, query heads per kv head, query tokens, keys, batch, head_dim: every workgroup walks many steps in each of
+# the three tile shapes; more keys than its table of pages of 16 keys holds; more of a tree than its table of
+# visibility words
+LONG = [(8, 4, 1, 6000, 16, 128), (8, 4, 30, 5000, 8, 128), (8, 8, 200, 3000, 2, 128),
+        (16, 8, 512, 17000, 1, 64), (16, 4, 30, 17000, 16, 64), (16, 1, 1, 40000, 8, 64), (16, 8, 700, 760, 1, 64)]
 
 
 @pytest.mark.parametrize("case", LONG, ids=[f"l{i}" for i in range(len(LONG))])
-def test_varlen_runs_longer_than_their_tables(case):
-    hkv, group, q_len, keys, batch = case
+def test_varlen_long_runs(case):
+    hkv, group, q_len, keys, batch, d = case
     print(f"[attend] {case}", flush=True)
     g = torch.Generator(device="cuda").manual_seed(q_len)
-    d, n = 64, batch * q_len
+    n = batch * q_len
     q = torch.randn(n, hkv * group, d, generator=g, device="cuda").to(BF)
     kv = torch.randn(batch, 2, hkv, keys, d, generator=g, device="cuda").to(BF)
     mask = su.tree_masks([q_len])[0].cuda()
     lens = dict(q_indptr=torch.arange(batch + 1, dtype=torch.int32, device="cuda") * q_len,
                 kv_lens=torch.full((batch,), keys, dtype=torch.int32, device="cuda"))
     outs = []
-    for page in (16, 1024):
+    for page in (16, 1024):  # each twice: a wait that is missing shows as a difference between runs
         pages = -(-keys // page)
         cache = torch.zeros(batch, 2, hkv, pages * page, d, dtype=BF, device="cuda")
         cache[:, :, :, :keys] = kv
         cache = cache.view(batch, 2, hkv, pages, page, d).permute(0, 3, 1, 2, 4, 5).reshape(-1, 2, hkv, page, d)
         table = torch.arange(batch * pages, dtype=torch.int32, device="cuda").view(batch, pages)
-        outs.append(tsf.tree_sparse_attention_fwd_paged_varlen(q, cache, table, mask, kv_layout="HND", **lens))
+        for _ in range(2):
+            outs.append(tsf.tree_sparse_attention_fwd_paged_varlen(q, cache, table, mask, kv_layout="HND", **lens))
         del cache
     torch.cuda.synchronize()
     # the pages' size changes where a run's tables end and nothing else
-    assert torch.equal(outs[0], outs[1])
-    # the last sequence's first and last kv head in 64 bits
-    for h in (0, hkv - 1):
-        k, v = kv[-1, 0, h].double(), kv[-1, 1, h].double()
-        x = q[n - q_len:, h * group:(h + 1) * group].double().transpose(0, 1).reshape(-1, d)
-        score = (x @ k.t()) * d ** -0.5
-        most = float((x.abs() @ k.abs().t()).max()) * d ** -0.5
-        score = score.view(group, q_len, keys)
-        score[:, :, keys - q_len:].masked_fill_(~mask, -torch.inf)
-        w = torch.softmax(score, -1).view(-1, keys)
-        ref, size = w @ v, w @ v.abs()
-        got = outs[0][n - q_len:, h * group:(h + 1) * group].double().transpose(0, 1).reshape(-1, d)
-        assert bool(((got - ref).abs() <= so.attention_tolerance(ref, size, most, BF, keys)).all())
+    for out in outs[1:]:
+        assert torch.equal(outs[0], out)
+    # sequences and kv heads in 64 bits
+    for b in {0, batch // 2, batch - 1}:
+        for h in range(hkv) if keys < 10000 else (0, hkv - 1):
+            k, v = kv[b, 0, h].double(), kv[b, 1, h].double()
+            rows, heads = slice(b * q_len, (b + 1) * q_len), slice(h * group, (h + 1) * group)
+            x = q[rows, heads].double().transpose(0, 1).reshape(-1, d)
+            score = (x @ k.t()) * d ** -0.5
+            most = float((x.abs() @ k.abs().t()).max()) * d ** -0.5
+            score = score.view(group, q_len, keys)
+            score[:, :, keys - q_len:].masked_fill_(~mask, -torch.inf)
+            w = torch.softmax(score, -1).view(-1, keys)
+            ref, size = w @ v, w @ v.abs()
+            got = outs[0][rows, heads].double().transpose(0, 1).reshape(-1, d)
+            assert bool(((got - ref).abs() <= so.attention_tolerance(ref, size, most, BF, keys)).all())
 
 
 @pytest.mark.parametrize("sm_scale", [0.0, -0.2, 3.0])
