@@ -105,8 +105,8 @@ template <int N> __device__ inline void dma_rows(const void* base, const uint32_
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_in);
   if constexpr (N == 4)
     asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\t"
-                 "global_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
+                 "global_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:0x400\n\t"
+                 "global_load_lds_dwordx4 %2, %4 offset:0x800\n\tglobal_load_lds_dwordx4 %3, %4 offset:0xc00"
                  :
                  : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(sbase), "s"(lds)
                  : "memory", "m0");
@@ -117,7 +117,7 @@ template <int N> __device__ inline void dma_rows(const void* base, const uint32_
                  : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\t"
-                 "global_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                 "global_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x400"
                  :
                  : "v"(off[0]), "v"(off[1]), "s"(sbase), "s"(lds)
                  : "memory", "m0");
@@ -923,16 +923,35 @@ struct Sizes {
   size_t total() const { return o + ml + runs + desc; }
 };
 
-// Tiles by the rows (query token x head of a kv head) of a sequence on
-// average: 32 rows and four key streams up to 32 of them (decoding), 256 rows
-// and one stream above 512, else 128 rows and two.
-inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim) {
+// Rows of a tile, by the rows of a sequence (query token x head of a kv head)
+// and by the work: the steps of 32 rows x 128 keys that a workgroup would take,
+// sequences and lists (`keys` of them to a sequence) at their mean.  32 rows and
+// four key streams for sequences of up to 32 rows, 128 rows and two streams for
+// longer ones; but
+// 32 rows too where there is little work, for such a tile starts and ends
+// sooner (and its tiles are few: a run that holds pieces of three loses that
+// again).  1 sequence, 8 kv heads, D 128, 128 / 256 rows: 2 steps 18.9 / 17.5
+// us against 24.9 / 23.0 with 128 rows, 4 steps 21.4 / 20.8 against 26.2 /
+// 24.3, 8 steps 27.8 / 26.2 against 27.0 / 27.8, 12 steps 32.0 / 31.5 against
+// 29.5 / 28.0;
+// 256 rows and one stream where there is much, for it reads the keys half as
+// often: 512 to 2048 rows of 16 sequences by 4096 keys (264 steps and more)
+// 160 to 675 us against 184 to 803 us, 8 x 1024 rows by 2300 (144 steps) 100
+// against 113, 8 x 512 rows by 2176 (68 steps) 62 against 57, 2048 rows by 4600
+// (72 steps) 69 against 65.
+constexpr int64_t kLittleWork = 8, kMuchWork = 128;  // steps
+constexpr int64_t kMaxKeys = 1 << 30;
+inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim, int64_t keys) {
   Sizes s;
-  const int64_t rows = (int64_t)total_q * (num_heads / num_kv_heads);
-  s.rows = rows <= (int64_t)32 * batch ? 32 : rows > (int64_t)512 * batch ? 256 : 128;
+  s.groups = cus < kMaxGroups ? cus : kMaxGroups;
+  const int64_t rows = (int64_t)total_q * (num_heads / num_kv_heads);  // <= 2^30
+  const int64_t tiles = (rows + 32 * (int64_t)batch - 1) / (32 * (int64_t)batch) * batch * num_kv_heads;
+  const double steps = (double)tiles * (double)(keys < kMaxKeys ? keys : kMaxKeys) / (128.0 * s.groups);
+  s.rows = rows <= (int64_t)32 * batch || (tiles <= s.groups * 3 / 4 && steps <= kLittleWork) ? 32
+           : rows > (int64_t)256 * batch && steps >= kMuchWork                               ? 256
+                                                                                              : 128;
   s.streams = s.rows == 32 ? 4 : s.rows == 256 ? 1 : 2;
   s.extra = s.rows == 32 ? 2 : 8;
-  s.groups = cus < kMaxGroups ? cus : kMaxGroups;
   s.o = align256((size_t)2 * s.groups * s.rows * head_dim * 4);
   s.ml = align256((size_t)2 * s.groups * s.rows * 8);
   s.runs = align256((size_t)s.groups * 4);
@@ -985,7 +1004,8 @@ extern "C" size_t tsfa_fwd_paged_varlen_workspace_bytes(int batch, int total_q, 
   if (varlen::check(batch, total_q, num_heads, num_kv_heads, head_dim, dtype) != TSFA_OK || batch == 0 || total_q == 0)
     return 0;
   if (device_cu_count(&cus) != TSFA_OK) return 0;
-  return varlen::sizes_of(cus, batch, total_q, num_heads, num_kv_heads, head_dim).total();
+  // the larger of the tiles a call with these rows may take
+  return varlen::sizes_of(cus, batch, total_q, num_heads, num_kv_heads, head_dim, varlen::kMaxKeys).total();
 }
 
 extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* o, float* lse, const uint8_t* mask,
@@ -1018,7 +1038,8 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
   if (q_indptr == nullptr || kv_lens == nullptr || kv_indices == nullptr) return TSFA_ERR_INVALID_ARGUMENT;
   int cus = 0;
   if (device_cu_count(&cus) != TSFA_OK) return TSFA_ERR_DEVICE;
-  const varlen::Sizes sz = varlen::sizes_of(cus, batch, total_q, num_heads, num_kv_heads, head_dim);
+  const int64_t keys = (kv_indptr != nullptr ? n_indices / batch : (int64_t)page_table_width) * page_size;
+  const varlen::Sizes sz = varlen::sizes_of(cus, batch, total_q, num_heads, num_kv_heads, head_dim, keys);
   if (workspace == nullptr || workspace_bytes < sz.total() || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return TSFA_ERR_WORKSPACE;
 

@@ -26,8 +26,9 @@ def _same(a, b):
 
 # ------------------------------------------------------------------ attention
 def _attend(q_lens, kv_lens, hq=8, hkv=2, d=128, dtype=BF, page=16, layout="NHD", mask="tree", dense=False, seed=0,
-            sm_scale=None, pad=0, stale=NAN, edit=None, check=True):
-    """One call against the plain form; returns what was used."""
+            sm_scale=None, pad=0, stale=NAN, edit=None, check=True, room=0):
+    """One call against the plain form; returns what was used.  ``room``: entries behind each page list's last page,
+    which the lengths do not reach."""
     g = torch.Generator().manual_seed(1000 + seed)
     n = sum(q_lens)
     cache, lists = su.pool(q_lens, kv_lens, hkv, d, dtype, page, layout, seed, stale=stale)
@@ -39,7 +40,7 @@ def _attend(q_lens, kv_lens, hq=8, hkv=2, d=128, dtype=BF, page=16, layout="NHD"
         tree = su.tree_masks([max(q_lens)], seed)[0]
     if edit is not None:
         edit(q, cache, lists, tree)
-    indices, indptr = su.tables(lists, dense)
+    indices, indptr = su.tables([list(x) + [0] * room for x in lists], dense)
     q_indptr, kl = su.lengths(q_lens, kv_lens)
     dq, dc, di, dp, dqi, dkl, dt = _dev(q, cache, indices, indptr, q_indptr, kl, tree)
     out = torch.full_like(dq, NAN)
@@ -92,19 +93,25 @@ ATTEND = [
 ]
 
 
+# Lists with room for few keys take tiles of 32 rows where a call is small, lists with room for many 128 or 256.
+ROOM = pytest.mark.parametrize("room", [0, 1 << 18], ids=["tight", "roomy"])
+
+
+@ROOM
 @pytest.mark.parametrize("case", ATTEND, ids=[f"a{i}" for i in range(len(ATTEND))])
-def test_varlen_attention(case):
+def test_varlen_attention(case, room):
     q_lens, kv_lens, kw = case
-    print(f"[attend] {q_lens} {kv_lens} {kw}", flush=True)
+    print(f"[attend] {q_lens} {kv_lens} {kw} room {room}", flush=True)
     # rows of the pool that hold no key are NaN: none may reach a result
-    _attend(q_lens, [max(a, b) for a, b in zip(q_lens, kv_lens)], seed=len(q_lens), **kw)
+    _attend(q_lens, [max(a, b) for a, b in zip(q_lens, kv_lens)], seed=len(q_lens), room=room, **kw)
 
 
 # kv heads, query heads per kv head, query tokens, keys, batch, head_dim: every workgroup walks many steps in each of
 # the three tile shapes; more keys than its table of pages of 16 keys holds; more of a tree than its table of
 # visibility words
-LONG = [(8, 4, 1, 6000, 16, 128), (8, 4, 30, 5000, 8, 128), (8, 8, 200, 3000, 2, 128),
-        (16, 8, 512, 17000, 1, 64), (16, 4, 30, 17000, 16, 64), (16, 1, 1, 40000, 8, 64), (16, 8, 700, 760, 1, 64)]
+LONG = [(8, 4, 1, 6000, 16, 128), (8, 4, 30, 5000, 8, 128), (8, 8, 200, 3000, 2, 128), (8, 8, 200, 4000, 4, 128),
+        (16, 8, 512, 17000, 1, 64), (16, 4, 30, 17000, 16, 64), (16, 1, 1, 40000, 8, 64), (16, 8, 700, 760, 1, 64),
+        (16, 8, 700, 760, 3, 64)]
 
 
 @pytest.mark.parametrize("case", LONG, ids=[f"l{i}" for i in range(len(LONG))])
@@ -148,30 +155,34 @@ def test_varlen_long_runs(case):
             assert bool(((got - ref).abs() <= so.attention_tolerance(ref, size, most, BF, keys)).all())
 
 
+@ROOM
 @pytest.mark.parametrize("sm_scale", [0.0, -0.2, 3.0])
-def test_varlen_scales(sm_scale):
-    print(f"[attend] scale {sm_scale}", flush=True)
-    _attend([10, 33], [90, 65], sm_scale=sm_scale)
+def test_varlen_scales(sm_scale, room):
+    print(f"[attend] scale {sm_scale} room {room}", flush=True)
+    _attend([10, 33], [90, 65], sm_scale=sm_scale, room=room)
 
 
-def test_varlen_rows_without_keys_are_zero():
-    print("[attend] empty rows", flush=True)
+@ROOM
+def test_varlen_rows_without_keys_are_zero(room):
+    print(f"[attend] empty rows room {room}", flush=True)
 
     def edit(q, cache, lists, tree):
         tree[0, 3] = False
         tree[1, 0] = False
 
-    s = _attend([6, 4], [6, 4], edit=edit)
+    s = _attend([6, 4], [6, 4], edit=edit, room=room)
     assert bool((s["out"][3] == 0).all()) and bool((s["out"][6] == 0).all())
     # behind a prefix the same rows see it
-    _attend([6, 4], [40, 37], edit=edit)
+    _attend([6, 4], [40, 37], edit=edit, room=room)
+    _attend([66, 80], [106, 100], edit=edit, room=room)
 
 
-def test_varlen_non_finite_values_in_masked_places():
-    print("[attend] masked NaN and infinities", flush=True)
+@ROOM
+def test_varlen_non_finite_values_in_masked_places(room):
+    print(f"[attend] masked NaN and infinities room {room}", flush=True)
     for dtype in (BF, FP):
         for bad in (NAN, float("inf"), -float("inf")):
-            for q_len, kv_len in ((40, 40), (40, 300)):
+            for q_len, kv_len in ((40, 40), (40, 300), (80, 300)):
                 def edit(q, cache, lists, tree):
                     # token 7 is seen by itself and its descendants alone
                     key = kv_len - q_len + 7
@@ -181,7 +192,7 @@ def test_varlen_non_finite_values_in_masked_places():
                     tree[0, 7, 7] = False
                     tree[0, 20, 7] = bad == bad  # one row sees the infinities
 
-                s = _attend([q_len], [kv_len], dtype=dtype, edit=edit, check=bad != bad)
+                s = _attend([q_len], [kv_len], dtype=dtype, edit=edit, check=bad != bad, room=room)
                 rows = [i for i in range(q_len) if i != 20 or bad != bad]
                 assert bool(s["out"][rows].isfinite().all())
                 assert not bool(s["out"][20].isfinite().all()) or bad != bad
@@ -239,9 +250,10 @@ def test_varlen_equals_the_uniform_paged_forward():
     assert float(diff.max()) <= bound
 
 
-def test_varlen_device_lengths_out_of_range_read_nothing_outside():
-    print("[attend] lengths and pages out of range", flush=True)
-    s = _attend([5, 9], [50, 95])
+@ROOM
+def test_varlen_device_lengths_out_of_range_read_nothing_outside(room):
+    print(f"[attend] lengths and pages out of range room {room}", flush=True)
+    s = _attend([5, 12], [50, 95], room=room)
     q, cache = s["q"], s["cache"].nan_to_num(0)
     put = dict(dtype=torch.int32, device="cuda")
     # a list with pages outside the pool, lengths past the list, negative and falling lengths
