@@ -12,13 +12,25 @@
 // One workgroup per CU takes an equal run of the call's steps (tsfa_paged.h);
 // what the run's first and last tile share with the neighbours' goes through
 // the workspace, in fp32, and combine_kernel joins it.  A workgroup's waves
-// are S key streams of RG row groups of 32 rows: S = 2, RG = 4 for trees
-// (128 rows share each key), S = 4, RG = 1 where a sequence has 32 rows or
-// fewer (decoding: every wave streams keys of its own).  A step is 32 S keys;
-// stream s takes 32 of them through its own LDS ring (global_load_lds, HBM ->
-// LDS without registers).  S^T = K Q^T and O^T += V^T P^T on
-// v_mfma_f32_32x32x16: a lane holds one query row in both, so the softmax
-// statistics stay in the lane, with one exchange between the lane halves.
+// are S key streams of RG row groups of 32 rows; a step is 32 S keys, of which
+// stream s takes 32 through its own LDS ring (global_load_lds, HBM -> LDS
+// without registers).  Three shapes, chosen in sizes_of:
+//   S = 4, RG = 1   32 rows: decoding and little work, every wave on keys of
+//                   its own, the streams joined in LDS;
+//   S = 2, RG = 4   128 rows: trees, four waves share each key;
+//   S = 1, RG = 8   256 rows: much work, K and V read half as often; half of a
+//                   SIMD's waves run one product behind the others.
+// S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: a lane holds one query
+// row in both, so the softmax statistics stay in the lane, with one exchange
+// between the lane halves.
+//
+// What bounds it: with 32 rows the reading of K and V (64 sequences of 500 to
+// 16384 keys, one token each: 1.17 GB in 228 us, 5.1 TB/s, a copy's rate); with
+// 128 and 256 rows the issue of matrix products beside the softmax (4 x 200 to
+// 256 tokens of 64 heads by 8192 to 32768 keys: 472 GFLOP in 560 us, 840 TFLOP/s,
+// where a large product reaches 1170 to 1220; MFMA busy 45 %); in calls of a few
+// steps the fixed part, 8 us until a run's first unit has arrived and 3 to 8 us
+// for the partial tiles' store and join.
 #include <hip/hip_runtime.h>
 
 #include <math.h>

@@ -260,7 +260,7 @@ int tsfa_fwd_paged(const void* q, const void* kv_cache, const int32_t* kv_indptr
  * strides    int64[12]: q, k, v, out -- (token, head, d) each, in elements;
  *            d strides 1, rows 16-byte aligned
  * Supported: fp16 / bf16; head_dim <= 256 and rot_dim <= head_dim, multiples
- * of 16.  Two tokens must not share a place in the pool. */
+ * of 16; total_q <= 2^23.  Two tokens must not share a place in the pool. */
 int tsfa_append_paged_kv(const void* q, const void* k, const void* v, void* out, void* kv_cache,
                          const void* positions, int positions_64, const float* inv_freq, int rot_dim,
                          int interleaved, float attention_scaling, const int32_t* q_indptr,
@@ -285,7 +285,8 @@ int tsfa_append_paged_kv(const void* q, const void* k, const void* v, void* out,
  * workspace  tsfa_fwd_paged_varlen_workspace_bytes, 16-byte aligned; its size
  *            does not depend on the lengths
  * Supported: fp16 / bf16, head_dim 64 or 128, num_heads a multiple of
- * num_kv_heads (at most 256 times), up to 2^30 keys per sequence. */
+ * num_kv_heads (at most 256 times), total_q * (num_heads / num_kv_heads) <=
+ * 2^30, up to 2^30 keys per sequence; cache rows at least head_dim apart. */
 size_t tsfa_fwd_paged_varlen_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads, int head_dim,
                                              int dtype);
 int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* o, float* lse, const uint8_t* mask,
@@ -311,7 +312,8 @@ int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* o, float* l
  * states     n_states (at most 8) host pointers to [batch, beams] dense rows
  *            of state_row_bytes bytes, copied to out_states [batch, k]
  * Supported: k <= 64 (and <= beams * vocab), beams <= 256, beams * vocab <=
- * 2^30.  workspace 16-byte aligned. */
+ * 2^30, batch * k <= 2^23, and up to 2^23 tiles (2048 to 8192 logits of a row
+ * each).  workspace 16-byte aligned. */
 size_t tsfa_beam_select_workspace_bytes(int batch, int beams, int vocab, int k);
 int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, int64_t logits_beam_stride,
                      const float* scores, int64_t scores_seq_stride, int64_t scores_beam_stride, int batch,
