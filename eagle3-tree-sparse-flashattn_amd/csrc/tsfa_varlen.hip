@@ -142,6 +142,21 @@ __device__ inline float max3f(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// The largest of 16 scores.  One block: between blocks the compiler waits a
+// cycle for what it cannot see in them.  It cannot see either that a matrix
+// product may just have written them: FRESH waits for that (11 cycles).
+template <bool FRESH> __device__ inline float max16f(const f32x16& s) {
+  float r, t0, t1, t2, t3;
+  if constexpr (FRESH) asm volatile("s_nop 15" ::"v"(s));
+  asm volatile(
+      "v_max3_f32 %0, %5, %6, %7\n\tv_max3_f32 %1, %8, %9, %10\n\tv_max3_f32 %2, %11, %12, %13\n\t"
+      "v_max3_f32 %3, %14, %15, %16\n\tv_max3_f32 %4, %17, %18, %19\n\tv_max3_f32 %0, %0, %1, %20\n\t"
+      "v_max3_f32 %2, %2, %3, %4\n\tv_max_f32 %0, %0, %2"
+      : "=&v"(r), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+      : "v"(s[0]), "v"(s[1]), "v"(s[2]), "v"(s[3]), "v"(s[4]), "v"(s[5]), "v"(s[6]), "v"(s[7]), "v"(s[8]), "v"(s[9]),
+        "v"(s[10]), "v"(s[11]), "v"(s[12]), "v"(s[13]), "v"(s[14]), "v"(s[15]));
+  return r;
+}
 template <int N> __device__ inline void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 // At most `left` units of LPW loads each still on their way (left <= K).
 template <int LPW, int K> __device__ inline void wait_units(int left) {
@@ -351,7 +366,9 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-    float m_run = -INFINITY, m_lim = -INFINITY, l_run = 0.f;
+    // the reference point of the exponentials, where it has to move, it times
+    // the scale, the sum
+    float m_run = -INFINITY, m_lim = -INFINITY, ms = 0.f, l_run = 0.f;
     const float thr = kRescaleLog2 / sl2;
 
     const char* hbase = reinterpret_cast<const char*>(static_cast<const T*>(a.cache) + pl.kvh * a.ch);
@@ -401,10 +418,10 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           next_page[x] = table[min((min(k0 + 16 * ((rg * LPW / GL + x) & 1), kl - 1) >> ps) - first_page, kTableIds - 1)];
       };
       peek(0);
-      auto issue = [&](int j) {
+      auto issue = [&](auto whole_c, int j) {  // whole: the unit ends within the keys
         const int k0 = ((c0 + j) * S + st) * 32;
         const uint32_t dst = ring + (uint32_t)j % NST * C::kUnit;
-        if (k0 + 32 <= kl) {
+        if (decltype(whole_c)::value || k0 + 32 <= kl) {
 #pragma unroll
           for (int x = 0; x < NG; ++x) {
             const uint32_t row = (uint32_t)(k0 + 16 * ((rg * LPW / GL + x) & 1)) & ((1u << ps) - 1u);
@@ -457,17 +474,18 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         return s;
       };
       auto none = [](auto...) {};
+      constexpr std::true_type full{};
+      constexpr std::false_type part{};
       int issued = 0;
 
       // Unit j, whose scores are in s: its row statistics and P (rounded pairs
       // in pk), O re-based where needed.  NEXT: a unit that every row sees
       // whole, unit j + 1's scores (left in s) between its exponentials; else
-      // the unit may need its mask (w: the row's visible keys).
-      auto soft = [&](auto next_c, int j, f32x16& s, uint32_t (&pk)[8], uint32_t& w) {
-        constexpr bool NEXT = decltype(next_c)::value;
+      // the unit may need its mask (w: the row's visible keys).  STEADY: one
+      // unit is due, and it ends within the keys.
+      auto soft = [&](auto next_c, auto steady_c, int j, f32x16& s, uint32_t (&pk)[8], uint32_t& w) {
+        constexpr bool NEXT = decltype(next_c)::value, STEADY = decltype(steady_c)::value;
         const int u = (c0 + j) * S + st;
-        float alpha, ms;
-        bool need;
         auto stats = [&]() {
           if (!NEXT && (u + 1) * 32 > seen_by_all) {
             w = a.mask != nullptr ? words[(u - ut0) * M + rg * 32 + ln] : word_of(u * 32, t);
@@ -475,20 +493,22 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
             for (int i = 0; i < 16; ++i)
               if (!((w >> (8 * (i >> 2) + 4 * lh + (i & 3))) & 1u)) s[i] = -INFINITY;
           }
-          float mx = max3f(s[0], s[1], s[2]);
-#pragma unroll
-          for (int i = 3; i < 15; i += 2) mx = max3f(mx, s[i], s[i + 1]);
-          mx = max3f(mx, s[15], s[15]);
+          const float mx = max16f<!NEXT>(s);
           const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-          const float rmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          const float rmax = max3f(__uint_as_float(sw[0]), __uint_as_float(sw[1]), __uint_as_float(sw[1]));
           // the reference point moves only when a score passes it by more than
           // 2^8 (exact for any consistent point; p stays below 2^8)
-          need = rmax > m_lim;
-          const float m_new = need ? rmax : m_run;
-          alpha = need ? __builtin_amdgcn_exp2f((m_run - m_new) * sl2) : 1.f;
-          m_run = m_new;
-          m_lim = m_new + thr;
-          ms = m_new == -INFINITY ? 0.f : m_new * sl2;
+          const bool need = rmax > m_lim;
+          if (__ballot(need) != 0) {
+            const float m_new = need ? rmax : m_run;
+            const float alpha = need ? __builtin_amdgcn_exp2f((m_run - m_new) * sl2) : 1.f;
+            m_run = m_new;
+            m_lim = m_new + thr;
+            ms = m_new == -INFINITY ? 0.f : m_new * sl2;
+            l_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+          }
         };
         // P is rounded to the input type for the product with V, which takes
         // 16-bit operands; its row sum takes the unrounded values.  Pinned where
@@ -504,7 +524,8 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         };
         if constexpr (NEXT) {
           const f32x16 sn = scores(smem + (st * NST + (uint32_t)(j + 1) % NST) * C::kUnit, [&]() {
-            while (issued < min(n, j + NST - STAG)) issue(issued++);
+            if constexpr (STEADY) issue(full, issued++);
+            else while (issued < min(n, j + NST - STAG)) issue(part, issued++);
             stats();
           }, [&](int kk) {
 #pragma unroll
@@ -516,11 +537,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) expo(i);
         }
-        l_run = l_run * alpha + psum;
-        if (__ballot(need) != 0) {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-        }
+        l_run += psum;
       };
 
       // O^T += V^T P^T of unit j.  V^T by the transposing LDS read: lane i of
@@ -601,7 +618,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
                        (((lane % CPR) ^ swz_k<D>(row)) << 3);
         dma_1k_rows(src, lds_addr(smem) + q_place<C>((wave * C::kQLoads + i) * 1024));
       }
-      while (issued < C::kAhead && issued < n) issue(issued++);
+      while (issued < C::kAhead && issued < n) issue(part, issued++);
       if (a.mask != nullptr) {
         // under the first units' way here; the barriers below order them
         for (int i = tid; i < (c1 * S - ut0) * M; i += C::kWaves * 64) {
@@ -622,12 +639,10 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
       if constexpr (C::kAhead < 2) {
         // unit 1 takes Q's stage: it has to be on its way before step 1 waits
         barrier();
-        while (issued < min(n, NST)) issue(issued++);
+        while (issued < min(n, NST)) issue(part, issued++);
       }
       f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
       uint32_t pk[8], w = 0xffffffffu;
-      constexpr std::true_type full{};
-      constexpr std::false_type part{};
       if constexpr (PIPE) {
         // Steps whose units every row of the tile sees whole.  Past barrier j
         // unit j + 1 is there, and every wave is done with unit j - 1 (with
@@ -636,27 +651,35 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         // its exponentials while they run it, and the other way round.
         const int n_full = min(n, seen_by_all / (32 * S) - c0);
         const bool late = STAG != 0 && rg >= RG / 2;
-        auto meet = [&](int i) {
-          if (i > 0 && issued < n) vm_wait<(NST - 3 - STAG) * LPW>();  // issued = i + NST - 1 - STAG
+        auto meet = [&](auto steady_c, int i) {
+          if (decltype(steady_c)::value) vm_wait<(NST - 3 - STAG) * LPW>();  // issued = i + NST - 1 - STAG
           else wait_units<LPW, NST - 3>(issued - 2 - i);
           barrier();
         };
-        if (late && n_full > 1) meet(0);
-        for (; j + 1 < n_full; ++j) {
-          if (!late) meet(j);
-          soft(full, j, s, pk, w);
-          if (late && j + 2 < n_full) meet(j + 1);
+        auto step = [&](auto steady_c) {
+          if (!late) meet(steady_c, j);
+          soft(full, steady_c, j, s, pk, w);
+          if (late && (decltype(steady_c)::value || j + 2 < n_full)) meet(steady_c, j + 1);
           pv(full, j, pk, w);
+          ++j;
+        };
+        // Steady from step 1 on, while every step requests one unit that ends
+        // within the keys: what is on its way is a constant then.
+        const int n_steady = min(n_full - 2, min(n, kl / (32 * S) - c0) - (NST - 1 - STAG));
+        if (late && n_full > 1) meet(part, 0);
+        while (j + 1 < n_full) {
+          step(part);
+          while (j < n_steady) step(full);
         }
       }
       for (;;) {
         w = 0xffffffffu;
-        soft(part, j, s, pk, w);
+        soft(part, part, j, s, pk, w);
         pv(part, j, pk, w);
         if (++j >= n) break;
         wait_units<LPW, NST - 2>(issued - 1 - j);
         barrier();  // unit j is there, and every wave is done with unit j - 1
-        while (issued < min(n, j + NST)) issue(issued++);
+        while (issued < min(n, j + NST)) issue(part, issued++);
         s = scores(smem + (st * NST + (uint32_t)j % NST) * C::kUnit, none, none);
       }
       barrier();  // the rings, the table and the words are free again
