@@ -165,7 +165,7 @@ extern "C" int tsfa_append_paged_kv(const void* q, const void* k, const void* v,
     if (p == nullptr) return TSFA_ERR_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return TSFA_ERR_UNSUPPORTED;
   }
-  if (positions == nullptr || q_indptr == nullptr || kv_lens == nullptr || kv_indices == nullptr ||
+  if (positions == nullptr || q_indptr == nullptr || kv_lens == nullptr || (kv_indices == nullptr && n_indices > 0) ||
       (rot_dim > 0 && inv_freq == nullptr))
     return TSFA_ERR_INVALID_ARGUMENT;
 

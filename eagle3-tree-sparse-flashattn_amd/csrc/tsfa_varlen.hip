@@ -1070,7 +1070,8 @@ extern "C" int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* 
     if (p == nullptr) return TSFA_ERR_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return TSFA_ERR_UNSUPPORTED;
   }
-  if (q_indptr == nullptr || kv_lens == nullptr || kv_indices == nullptr) return TSFA_ERR_INVALID_ARGUMENT;
+  if (q_indptr == nullptr || kv_lens == nullptr || (kv_indices == nullptr && n_indices > 0))
+    return TSFA_ERR_INVALID_ARGUMENT;
   int cus = 0;
   if (device_cu_count(&cus) != TSFA_OK) return TSFA_ERR_DEVICE;
   const int64_t keys = (kv_indptr != nullptr ? n_indices / batch : (int64_t)page_table_width) * page_size;

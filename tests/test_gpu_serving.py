@@ -40,6 +40,7 @@ def _attend(q_lens, kv_lens, hq=8, hkv=2, d=128, dtype=BF, page=16, layout="NHD"
         tree = su.tree_masks([max(q_lens)], seed)[0]
     if edit is not None:
         edit(q, cache, lists, tree)
+    room = min(room, (1 << 22) // len(lists))
     indices, indptr = su.tables([list(x) + [0] * room for x in lists], dense)
     q_indptr, kl = su.lengths(q_lens, kv_lens)
     dq, dc, di, dp, dqi, dkl, dt = _dev(q, cache, indices, indptr, q_indptr, kl, tree)
@@ -90,6 +91,10 @@ ATTEND = [
     ([40], [2100], dict(dtype=FP)),                                          # 128-row tiles, many steps
     ([150, 140], [1050, 1640], dict(hq=8, hkv=1)),                           # 256-row tiles, many steps
     ([90], [700], dict(hq=8, hkv=1, d=64, mask="causal", layout="HND")),
+    ([1, 3], [300, 40], dict(hq=256, hkv=1, d=64, mask="causal")),           # more heads than a tile has rows
+    ([5, 2, 1], [70, 130, 1], dict(hq=71, hkv=1, dtype=FP)),
+    ([1 + i % 2 for i in range(1500)], [1 + 7 * i % 50 for i in range(1500)],
+     dict(hq=2, hkv=1, d=64, mask="causal", page=32)),                       # many sequences
 ]
 
 
@@ -270,6 +275,23 @@ def test_varlen_device_lengths_out_of_range_read_nothing_outside(room):
                                                          out=torch.zeros_like(q))
         torch.cuda.synchronize()
         assert bool(out.isfinite().all())
+
+
+@ROOM
+def test_varlen_sequences_without_any_key(room):
+    print(f"[attend] sequences without keys room {room}", flush=True)
+    q = torch.randn(40, 8, 64, generator=torch.Generator().manual_seed(1)).to(BF)
+    cache, _ = su.pool([1], [16], 2, 64, BF, 16, stale=NAN)
+    cache.fill_(NAN)
+    put = dict(dtype=torch.int32, device="cuda")
+    rows, none = torch.tensor([0, 3, 3, 38], **put), torch.zeros(3, **put)
+    for indices, indptr in ((torch.zeros(3 * (1 + room), **put), torch.arange(4, **put) * (1 + room)),
+                            (torch.zeros(0, **put), torch.zeros(4, **put)), (torch.zeros(3, 2, **put), None)):
+        out, lse = tsf.tree_sparse_attention_fwd_paged_varlen(
+            q.cuda(), cache.cuda(), indices, q_indptr=rows, kv_lens=none, kv_indptr=indptr,
+            out=torch.full((40, 8, 64), 3.0, dtype=BF, device="cuda"), return_lse=True)
+        torch.cuda.synchronize()
+        assert bool((out[:38] == 0).all()) and bool((lse[:38] == -torch.inf).all()) and bool((out[38:] == 3).all())
 
 
 def test_varlen_fewer_keys_than_queries():
