@@ -14,9 +14,10 @@
 //   merge_kernel  one workgroup per b: lse of every beam, the k best of the
 //                 tiles' candidates;
 //   states_kernel the states' rows of the selected parents.
-// The vocabulary pass is bound by memory and nearly as much by its exponentials
-// of 64 bits: 64 x 8 rows of 128256 fp32 logits (263 MB) take 70 us, 3.8 TB/s,
-// where a copy reaches 5.1.  4 x 10 rows of fp16 (10 MB) take 12 us and 12 us of
+// The vocabulary pass is bound by its exponentials of 64 bits (thirteen
+// operations of 64 bits a logit; fp16 and fp32 logits take the same time), then
+// by memory: 64 x 8 rows of 128256 fp32 logits (263 MB) take 64 us, 4.1 TB/s,
+// where a copy reaches 5.1.  4 x 10 rows of fp16 (10 MB) take 12 us and 11 us of
 // merge, one row of 32000 takes 6 and 8 us: there the time is that of the
 // launches and of a chain of loads and barriers.
 #include <hip/hip_runtime.h>
@@ -33,7 +34,6 @@ constexpr int kThreads = 256;
 constexpr int kMaxK = 64;
 constexpr int kMaxBeams = 256;
 constexpr int kMaxStates = 8;
-constexpr int kFullCard = 512;  // workgroups, see elements_per_thread
 constexpr int64_t kStatesInside = 128 << 10;  // bytes of a sequence's selected states, see tsfa_beam_select
 constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch
 
@@ -488,14 +488,15 @@ __global__ __launch_bounds__(kThreads) void states_kernel(const States st, const
            (int64_t)gridDim.y * kThreads);
 }
 
-// Elements of a tile per thread: long tiles, which leave the merge fewer
-// candidates, where they fill the card, short ones where a row has to be spread
-// over it.  4 x 10 rows of 128256 fp16 logits: 32 elements (640 tiles) 11.7 us
-// and 11.6 us of merge, 16 elements 11.2 and 12.4 us, 8 elements 12.9 and 16.7
-// us.
+// Elements of a tile per thread: long tiles, whose fixed part (reductions, the
+// bound, the list) counts less and which leave the merge fewer candidates,
+// where they fill the card, short ones where a row has to be spread over it.
+// 128256 fp16 logits a row, the whole call: 64 x 8 rows 74 us with 64 elements,
+// 79 with 32, 95 with 16; 16 x 4 rows (512 tiles of 64) 21.5 and 24; 4 x 10 rows
+// (320) 23.8 and 22.1, with 8 elements 27.
 inline int elements_per_thread(int64_t rows, int vocab) {
-  for (int ept = 32; ept > 8; ept /= 2)
-    if (rows * (((int64_t)vocab + kThreads * ept - 1) / (kThreads * ept)) >= kFullCard) return ept;
+  for (int ept = 64; ept > 8; ept /= 2)
+    if (rows * (((int64_t)vocab + kThreads * ept - 1) / (kThreads * ept)) >= 512) return ept;
   return 8;
 }
 inline int64_t tiles_of(int64_t rows, int vocab) {
@@ -516,7 +517,8 @@ int check(int batch, int beams, int vocab, int k, int dtype) {
 template <typename T> void launch_part(const PartArgs& a, int ept, int64_t rows, hipStream_t s) {
   const dim3 grid((unsigned)(rows * a.tiles));
   const size_t lds = (size_t)a.k * ept * sizeof(uint64_t);
-  if (ept == 32) hipLaunchKernelGGL((part_kernel<T, 32>), grid, dim3(kThreads), lds, s, a);
+  if (ept == 64) hipLaunchKernelGGL((part_kernel<T, 64>), grid, dim3(kThreads), lds, s, a);
+  else if (ept == 32) hipLaunchKernelGGL((part_kernel<T, 32>), grid, dim3(kThreads), lds, s, a);
   else if (ept == 16) hipLaunchKernelGGL((part_kernel<T, 16>), grid, dim3(kThreads), lds, s, a);
   else hipLaunchKernelGGL((part_kernel<T, 8>), grid, dim3(kThreads), lds, s, a);
 }

@@ -312,7 +312,7 @@ int tsfa_fwd_paged_varlen(const void* q, const void* kv_cache, void* o, float* l
  * states     n_states (at most 8) host pointers to [batch, beams] dense rows
  *            of state_row_bytes bytes, copied to out_states [batch, k]
  * Supported: k <= 64 (and <= beams * vocab), beams <= 256, beams * vocab <=
- * 2^30, batch * k <= 2^23, and up to 2^23 tiles (2048 to 8192 logits of a row
+ * 2^30, batch * k <= 2^23, and up to 2^23 tiles (2048 to 16384 logits of a row
  * each).  workspace 16-byte aligned. */
 size_t tsfa_beam_select_workspace_bytes(int batch, int beams, int vocab, int k);
 int tsfa_beam_select(const void* logits, int64_t logits_seq_stride, int64_t logits_beam_stride,

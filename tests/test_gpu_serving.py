@@ -500,7 +500,8 @@ def _select(logits, scores, k, states=()):
 @pytest.mark.parametrize("dtype", [BF, FP, torch.float32], ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("batch,beams,vocab,k", [(1, 1, 1, 1), (2, 1, 7, 7), (1, 1, 32000, 8), (3, 5, 1001, 10),
                                                  (2, 10, 9000, 64), (1, 64, 2049, 33), (5, 2, 8193, 1),
-                                                 (130, 8, 515, 8), (1, 256, 40, 64)])
+                                                 (130, 8, 515, 8), (1, 256, 40, 64), (52, 5, 20000, 10), (16, 8, 40001, 20),
+                                                 (6, 10, 36000, 64)])
 def test_select(dtype, batch, beams, vocab, k):
     print(f"[select] {dtype} {batch} {beams} {vocab} {k}", flush=True)
     logits, scores = _logits(batch, beams, vocab, dtype, seed=vocab + k)
@@ -540,6 +541,12 @@ def test_select_more_ties_than_a_round_holds():
     scores = torch.full((2, 64), -1.0)
     logits[1, 5:, 7] = 3.0  # and ties at the top
     _select(logits, scores, 64)
+    for batch, beams, vocab in ((2, 256, 2100), (2, 64, 33000), (4, 15, 36000)):  # rows for tiles of each length
+        logits = torch.full((batch, beams, vocab), -0.5, dtype=FP)
+        scores = torch.zeros(batch, beams)
+        scores[1, 7] = 0.25
+        for k in (1, 3):
+            _select(logits, scores, k)
 
 
 def test_select_logits_past_32_bit_offsets():
