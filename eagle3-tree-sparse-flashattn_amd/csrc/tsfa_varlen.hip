@@ -959,32 +959,33 @@ struct Sizes {
 };
 
 // Rows of a tile, by the rows of a sequence (query token x head of a kv head)
-// and by the work: the steps of 32 rows x 128 keys that a workgroup would take,
-// sequences and lists (`keys` of them to a sequence) at their mean.  32 rows and
-// four key streams for sequences of up to 32 rows, 128 rows and two streams for
-// longer ones; but
-// 32 rows too where there is little work, for such a tile starts and ends
-// sooner (and its tiles are few: a run that holds pieces of three loses that
-// again).  1 sequence, 8 kv heads, D 128, 128 / 256 rows: 2 steps 18.9 / 17.5
-// us against 24.9 / 23.0 with 128 rows, 4 steps 21.4 / 20.8 against 26.2 /
-// 24.3, 8 steps 27.8 / 26.2 against 27.0 / 27.8, 12 steps 32.0 / 31.5 against
-// 29.5 / 28.0;
-// 256 rows and one stream where there is much, for it reads the keys half as
-// often: 512 to 2048 rows of 16 sequences by 4096 keys (264 steps and more)
-// 160 to 675 us against 184 to 803 us, 8 x 1024 rows by 2300 (144 steps) 100
-// against 113, 8 x 512 rows by 2176 (68 steps) 62 against 57, 2048 rows by 4600
-// (72 steps) 69 against 65.
-constexpr int64_t kLittleWork = 8, kMuchWork = 128;  // steps
+// and by the work: the steps of 128 rows x 64 keys that a workgroup would take,
+// sequences and lists (`keys` of them to a sequence) at their mean.
+// 32 rows and four key streams for sequences of up to 32 rows, and where there
+// is little work, for such a tile starts and ends sooner: up to 4.5 steps, or
+// 12 where two tiles of 32 rows read the keys as often as one of 128 (and while
+// the tiles are few: a run that holds pieces of three loses that again).
+// 128 rows and two streams above.  Time with 128 rows over time with 32, D 128,
+// at 2, 3, 4 and 5 steps: 128 rows a sequence 1.25 1.13 1.03 0.96, 256 rows 1.21
+// 1.18 1.12 1.04, 192 rows 1.13 1.03 0.98 0.92; 64 rows at 4, 8 and 11 steps 1.23
+// 1.15 1.05; D 64 1.04 to 1.29 at all of these.
+// 256 rows and one stream where there is much work, for it reads the keys half
+// as often: 512 to 2048 rows of 16 sequences by 4096 keys (132 steps and more)
+// 160 to 675 us against 184 to 803 us with 128 rows, 8 x 1024 rows by 2300 (72
+// steps) 100 against 113, 8 x 512 rows by 2176 (34 steps) 62 against 57, 2048 rows
+// by 4600 (36 steps) 69 against 65.
+constexpr double kLittleWork = 4.5, kLittleWork64 = 12, kMuchWork = 64;  // steps
 constexpr int64_t kMaxKeys = 1 << 30;
 inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim, int64_t keys) {
   Sizes s;
   s.groups = cus < kMaxGroups ? cus : kMaxGroups;
   const int64_t rows = (int64_t)total_q * (num_heads / num_kv_heads);  // <= 2^30
-  const int64_t tiles = (rows + 32 * (int64_t)batch - 1) / (32 * (int64_t)batch) * batch * num_kv_heads;
-  const double steps = (double)tiles * (double)(keys < kMaxKeys ? keys : kMaxKeys) / (128.0 * s.groups);
-  s.rows = rows <= (int64_t)32 * batch || (tiles <= s.groups * 3 / 4 && steps <= kLittleWork) ? 32
-           : rows > (int64_t)256 * batch && steps >= kMuchWork                               ? 256
-                                                                                              : 128;
+  // tiles of n rows
+  auto tiles = [&](int64_t n) { return (rows + n * batch - 1) / (n * batch) * batch * num_kv_heads; };
+  const double steps = (double)tiles(128) * (double)(keys < kMaxKeys ? keys : kMaxKeys) / (64.0 * s.groups);
+  const bool little = tiles(32) <= s.groups * 3 / 4 &&
+                      steps <= (rows <= (int64_t)64 * batch ? kLittleWork64 : kLittleWork);
+  s.rows = rows <= (int64_t)32 * batch || little ? 32 : rows > (int64_t)256 * batch && steps >= kMuchWork ? 256 : 128;
   s.streams = s.rows == 32 ? 4 : s.rows == 256 ? 1 : 2;
   s.extra = s.rows == 32 ? 2 : 8;
   s.o = align256((size_t)2 * s.groups * s.rows * head_dim * 4);
