@@ -168,6 +168,12 @@ template <int LPW, int K> __device__ inline void wait_units(int left) {
   }
 }
 __device__ inline void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// The same among the waves of a stream; ALONE: one wave, which waits for what
+// it reads.
+template <bool ALONE> __device__ inline void stream_barrier() {
+  if constexpr (ALONE) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  else barrier();
+}
 
 __device__ inline int64_t uniform64(int64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
@@ -636,11 +642,11 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
           qf[kk] = *reinterpret_cast<const i16x8*>(qt + (((2 * kk + lh) ^ swz_k<D>(ln)) << 4)) ^
                    (short)(a.neg_q ? 0x8000 : 0);
       }
-      if constexpr (C::kAhead < 2) {
-        // unit 1 takes Q's stage: it has to be on its way before step 1 waits
-        barrier();
+      if constexpr (RG == 1) barrier();  // below, a stream's ring and steps are its wave's own
+      // unit 1 takes Q's stage: it has to be on its way before step 1 waits
+      static_assert(C::kAhead >= 2 || RG == 1, "Q is read");
+      if constexpr (C::kAhead < 2)
         while (issued < min(n, NST)) issue(part, issued++);
-      }
       f32x16 s = scores(smem + st * NST * C::kUnit, none, none);
       uint32_t pk[8], w = 0xffffffffu;
       if constexpr (PIPE) {
@@ -654,7 +660,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         auto meet = [&](auto steady_c, int i) {
           if (decltype(steady_c)::value) vm_wait<(NST - 3 - STAG) * LPW>();  // issued = i + NST - 1 - STAG
           else wait_units<LPW, NST - 3>(issued - 2 - i);
-          barrier();
+          stream_barrier<RG == 1>();
         };
         auto step = [&](auto steady_c) {
           if (!late) meet(steady_c, j);
@@ -678,7 +684,7 @@ __global__ __launch_bounds__(S * RG * 64) void varlen_kernel(const Args a) {
         pv(part, j, pk, w);
         if (++j >= n) break;
         wait_units<LPW, NST - 2>(issued - 1 - j);
-        barrier();  // unit j is there, and every wave is done with unit j - 1
+        stream_barrier<RG == 1>();  // unit j is there, and every wave is done with unit j - 1
         while (issued < min(n, j + NST)) issue(part, issued++);
         s = scores(smem + (st * NST + (uint32_t)j % NST) * C::kUnit, none, none);
       }
