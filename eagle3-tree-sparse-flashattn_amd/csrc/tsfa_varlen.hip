@@ -968,19 +968,20 @@ struct Sizes {
 // and by the work: the steps of 128 rows x 64 keys that a workgroup would take,
 // sequences and lists (`keys` of them to a sequence) at their mean.
 // 32 rows and four key streams for sequences of up to 32 rows, and where there
-// is little work, for such a tile starts and ends sooner: up to 4.5 steps, or
-// 12 where two tiles of 32 rows read the keys as often as one of 128 (and while
-// the tiles are few: a run that holds pieces of three loses that again).
+// is little work, for such a tile starts and ends sooner: up to 5 steps, or 32
+// where two tiles of 32 rows read the keys as often as one of 128 (and while the
+// tiles are few: a run that holds pieces of three loses that again).
 // 128 rows and two streams above.  Time with 128 rows over time with 32, D 128,
-// at 2, 3, 4 and 5 steps: 128 rows a sequence 1.25 1.13 1.03 0.96, 256 rows 1.21
-// 1.18 1.12 1.04, 192 rows 1.13 1.03 0.98 0.92; 64 rows at 4, 8 and 11 steps 1.23
-// 1.15 1.05; D 64 1.04 to 1.29 at all of these.
+// at 2, 4, 5 and 6 steps: 96 rows a sequence 1.22 1.01 0.92 0.89, 128 rows 1.27
+// 1.09 1.05 1.03, 192 rows 1.12 1.01 0.97 0.93, 256 rows 1.25 1.17 1.11 1.04, D 64
+// 1.00 to 1.20 at all of these; 64 rows at 8, 16, 32 and 64 steps 1.18 1.09 0.99
+// 0.93, D 64 1.30 1.27 1.18 1.02.
 // 256 rows and one stream where there is much work, for it reads the keys half
 // as often: 512 to 2048 rows of 16 sequences by 4096 keys (132 steps and more)
 // 160 to 675 us against 184 to 803 us with 128 rows, 8 x 1024 rows by 2300 (72
 // steps) 100 against 113, 8 x 512 rows by 2176 (34 steps) 62 against 57, 2048 rows
 // by 4600 (36 steps) 69 against 65.
-constexpr double kLittleWork = 4.5, kLittleWork64 = 12, kMuchWork = 64;  // steps
+constexpr double kLittleWork = 5, kLittleWork64 = 32, kMuchWork = 64;  // steps
 constexpr int64_t kMaxKeys = 1 << 30;
 inline Sizes sizes_of(int cus, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim, int64_t keys) {
   Sizes s;
