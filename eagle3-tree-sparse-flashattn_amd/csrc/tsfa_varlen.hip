@@ -25,12 +25,13 @@
 // between the lane halves.
 //
 // What bounds it: with 32 rows the reading of K and V (64 sequences of 500 to
-// 16384 keys, one token each: 1.17 GB in 228 us, 5.1 TB/s, a copy's rate); with
-// 128 and 256 rows the issue of matrix products beside the softmax (4 x 200 to
-// 256 tokens of 64 heads by 8192 to 32768 keys: 472 GFLOP in 560 us, 840 TFLOP/s,
-// where a large product reaches 1170 to 1220; MFMA busy 45 %); in calls of a few
-// steps the fixed part, 8 us until a run's first unit has arrived and 3 to 8 us
-// for the partial tiles' store and join.
+// 16384 keys, one token each: 1.17 GB in 223 us, 5.2 TB/s, a copy's rate); with
+// 128 rows the reading of K and V for each of them and the issue of matrix
+// products beside the softmax, with 256 the issue alone (4 x 200 to 256 tokens of
+// 64 heads by 8192 to 32768 keys: 472 GFLOP in 520 us, 900 TFLOP/s, where a large
+// product reaches 1170 to 1220; MFMA busy 50 % at a power-limited clock); in
+// calls of a few steps the fixed part, 8 us until a run's first unit has arrived
+// and 3 to 8 us for the partial tiles' store and join.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
