@@ -989,7 +989,8 @@ def tree_sparse_attention_fwd_paged_varlen(q: torch.Tensor, kv_cache: torch.Tens
     return NaN there, as the reference does, but here such rows pad a batch
     and would carry the NaN into the cache.  Rows of ``out`` behind
     q_indptr[B] are left as they were (those of lse are not set).  Sequences
-    may share pages.  ``workspace`` (uint8,
+    may share pages.  The same call gives the same bits; a page list with more
+    room may take other tiles and so another order of the sums.  ``workspace`` (uint8,
     fwd_paged_varlen_workspace_bytes(...) bytes) must not be shared by calls
     that overlap in time, captured graphs among them.  No host
     synchronisation; page ids outside the pool are clamped (wrong O, never an

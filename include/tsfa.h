@@ -284,6 +284,9 @@ int tsfa_append_paged_kv(const void* q, const void* k, const void* v, void* out,
  * q_strides, o_strides  int64[3]: token, head, d
  * workspace  tsfa_fwd_paged_varlen_workspace_bytes, 16-byte aligned; its size
  *            does not depend on the lengths
+ * The same call gives the same bits.  How rows and keys are tiled follows
+ * total_q, batch, the heads and what the page lists could hold, so calls that
+ * differ there may differ in the order of their sums.
  * Supported: fp16 / bf16, head_dim 64 or 128, num_heads a multiple of
  * num_kv_heads (at most 256 times), total_q * (num_heads / num_kv_heads) <=
  * 2^30, up to 2^30 keys per sequence; cache rows at least head_dim apart. */
