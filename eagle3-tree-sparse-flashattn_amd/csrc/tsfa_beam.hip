@@ -409,7 +409,12 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
     }
     if (tid == 0) count = 0;
     if (c0 + kMergeThreads * kBatch < total) request(c0 + kMergeThreads * kBatch);
-    if (__syncthreads_or(top.value != 0) == 0) continue;
+    if (__syncthreads_or(top.value != 0) == 0) {
+      // a round that holds one of every list: what is behind it in its list is
+      // no better
+      if (lists <= kMergeThreads * kBatch) break;
+      continue;
+    }
     // as in part_kernel, by the upper half of the value: ties stay in
     const uint32_t hi[1] = {(uint32_t)(top.value >> 32)};
     const uint32_t wb = kth_order(hi, a.k);
