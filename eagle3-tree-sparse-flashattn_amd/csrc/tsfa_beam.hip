@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
   __shared__ double lse[kMaxBeams], score[kMaxBeams];
   __shared__ float tops[kMaxBeams];
   __shared__ Cand heads[kMergeThreads];
-  __shared__ Cand list[kMergeList];
+  __shared__ Cand list[2 * kMergeList];
   __shared__ Cand kept[kMaxK];
   __shared__ uint32_t wbound[NW];
   __shared__ Cand bound;
@@ -459,12 +459,31 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
     // the kept ones join, all are ranked, the k best stay
     for (int i = tid; i < a.k; i += kMergeThreads) list[n + i] = kept[i];
     __syncthreads();
-    for (int i = tid; i < n + a.k; i += kMergeThreads) {
-      const Cand x = list[i];
+    n += a.k;
+    int base = 0;
+    if (n > 2 * kMaxK) {
+      // The waves' bounds leave many where k is large (ranks are a list by a
+      // list: 35 beams, k = 31, 47 us of merge without this): once more by the
+      // bound of all of them, which each wave finds for itself.
+      uint32_t his[kMergeList / 64];
+#pragma unroll
+      for (int i = 0; i < kMergeList / 64; ++i)
+        his[i] = i * 64 + lane < n ? (uint32_t)(list[i * 64 + lane].value >> 32) : 0;
+      const uint32_t least = kth_order(his, a.k);
+      if (tid == 0) count = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += kMergeThreads)
+        if ((uint32_t)(list[i].value >> 32) >= least) list[kMergeList + atomicAdd(&count, 1)] = list[i];
+      __syncthreads();
+      base = kMergeList;
+      n = count;
+    }
+    for (int i = tid; i < n; i += kMergeThreads) {
+      const Cand x = list[base + i];
       if (x.value == 0) continue;
       int rank = 0;
 #pragma unroll 4
-      for (int j = 0; j < n + a.k; ++j) rank += better(list[j], x);
+      for (int j = 0; j < n; ++j) rank += better(list[base + j], x);
       if (rank < a.k) kept[rank] = x;
     }
     __syncthreads();
