@@ -416,8 +416,18 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const MergeArgs a)
       continue;
     }
     // as in part_kernel, by the upper half of the value: ties stay in
-    const uint32_t hi[1] = {(uint32_t)(top.value >> 32)};
-    const uint32_t wb = kth_order(hi, a.k);
+    uint32_t wb;
+    if (a.k <= 40) {
+      const uint32_t hi[1] = {(uint32_t)(top.value >> 32)};
+      wb = kth_order(hi, a.k);
+    } else {
+      // 64 threads' best leave too many: of all candidates (64 x 16 rows, k = 64:
+      // merge 21 us, by the threads' best 35; 9 x 35 rows, k = 31: 18 and 17)
+      uint32_t hi[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) hi[j] = (uint32_t)(cs[j].value >> 32);
+      wb = kth_order(hi, a.k);
+    }
     if (lane == 0) wbound[wave] = wb;
     __syncthreads();
     uint64_t lim = last.value > 1 ? last.value : 1;

@@ -501,7 +501,8 @@ def _select(logits, scores, k, states=()):
 @pytest.mark.parametrize("batch,beams,vocab,k", [(1, 1, 1, 1), (2, 1, 7, 7), (1, 1, 32000, 8), (3, 5, 1001, 10),
                                                  (2, 10, 9000, 64), (1, 64, 2049, 33), (5, 2, 8193, 1),
                                                  (130, 8, 515, 8), (1, 256, 40, 64), (52, 5, 20000, 10), (16, 8, 40001, 20),
-                                                 (6, 10, 36000, 64)])
+                                                 (6, 10, 36000, 64), (3, 35, 4778, 31),
+                                                 (1, 16, 160000, 64), (2, 11, 14164, 46)])
 def test_select(dtype, batch, beams, vocab, k):
     print(f"[select] {dtype} {batch} {beams} {vocab} {k}", flush=True)
     logits, scores = _logits(batch, beams, vocab, dtype, seed=vocab + k)
